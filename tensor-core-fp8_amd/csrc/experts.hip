@@ -1,0 +1,296 @@
+// C ABI of the operators for layers with experts: products of rows grouped by expert and their weight
+// gradient, quantisation of their operands, products with 4-bit weights (include/fp8gemm.h).  Validate,
+// pick a kernel, launch asynchronously, return the launch status.
+#include "fp8gemm.h"
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "dispatch.h"
+#include "kernel_quantize.h"
+#include "kernel_w4.h"
+
+namespace fp8gemm_detail {
+
+extern template hipError_t dispatch_grouped<0, 0>(int, int, int, const uint8_t *, const uint8_t *, void *, int, const GroupSpec &, hipStream_t);
+extern template hipError_t dispatch_grouped<0, 1>(int, int, int, const uint8_t *, const uint8_t *, void *, int, const GroupSpec &, hipStream_t);
+extern template hipError_t dispatch_grouped<1, 0>(int, int, int, const uint8_t *, const uint8_t *, void *, int, const GroupSpec &, hipStream_t);
+extern template hipError_t dispatch_grouped<1, 1>(int, int, int, const uint8_t *, const uint8_t *, void *, int, const GroupSpec &, hipStream_t);
+extern template hipError_t dispatch_wgrad<0, 0>(int, int, int, const uint8_t *, const uint8_t *, void *, int, const GroupSpec &, hipStream_t);
+extern template hipError_t dispatch_wgrad<0, 1>(int, int, int, const uint8_t *, const uint8_t *, void *, int, const GroupSpec &, hipStream_t);
+extern template hipError_t dispatch_wgrad<1, 0>(int, int, int, const uint8_t *, const uint8_t *, void *, int, const GroupSpec &, hipStream_t);
+extern template hipError_t dispatch_wgrad<1, 1>(int, int, int, const uint8_t *, const uint8_t *, void *, int, const GroupSpec &, hipStream_t);
+
+// ------------------------------------------------------------------ planning
+// The cut of the rows is known on the device only: the tile is chosen by the average rows of an expert.
+int plan_grouped(int m, int k, int n, int groups)
+{
+    const int average = (m + groups - 1) / groups;
+    if (average <= 64) return 15;
+    if (average <= 256 || !p2h_ok(k, 1)) return 6;
+    return 13;
+}
+
+int plan_wgrad(int m, int n, int rows, int groups)
+{
+    (void)rows;
+    const long tiles = (long)((m + 255) / 256) * ((n + 255) / 256) * groups;
+    return tiles >= 256 ? 13 : 6;
+}
+
+}  // namespace fp8gemm_detail
+
+using namespace fp8gemm_detail;
+
+namespace {
+
+static_assert(kMaxGroups == FP8GEMM_MAX_GROUPS, "the header names the table's size");
+
+bool fmt_ok(int f) { return f == FP8GEMM_E4M3 || f == FP8GEMM_E5M2; }
+bool wide_ok(int t) { return t == FP8GEMM_OUT_F32 || t == FP8GEMM_OUT_BF16 || t == FP8GEMM_OUT_F16; }
+bool aligned_to(const void *p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+// a place for elements of a wide type
+bool wide_aligned(const void *p, int type) { return aligned_to(p, type == FP8GEMM_OUT_F32 ? 4 : 2); }
+
+int grouped(int groups, int m, int k, int n, const int *row_offsets, const void *a, int a_fmt, const void *b, int b_fmt, void *out, int out_type,
+            const float *a_scale, const float *b_scale, int b_scale_per_column, int variant, void *stream)
+{
+    if (groups <= 0 || groups > kMaxGroups || m <= 0 || k <= 0 || n <= 0 || !row_offsets || !a || !b || !out) return (int)hipErrorInvalidValue;
+    if (!fmt_ok(a_fmt) || !fmt_ok(b_fmt) || !wide_ok(out_type) || !wide_aligned(out, out_type)) return (int)hipErrorInvalidValue;
+    const uint8_t *pa = static_cast<const uint8_t *>(a), *pb = static_cast<const uint8_t *>(b);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const GroupSpec spec = {row_offsets, groups, m, a_scale, b_scale, b_scale_per_column != 0, out_type, 0};
+    (void)hipGetLastError();
+    if (a_fmt == FP8GEMM_E4M3 && b_fmt == FP8GEMM_E4M3) return (int)dispatch_grouped<0, 0>(m, k, n, pa, pb, out, variant, spec, s);
+    if (a_fmt == FP8GEMM_E5M2 && b_fmt == FP8GEMM_E5M2) return (int)dispatch_grouped<1, 1>(m, k, n, pa, pb, out, variant, spec, s);
+    if (a_fmt == FP8GEMM_E4M3) return (int)dispatch_grouped<0, 1>(m, k, n, pa, pb, out, variant, spec, s);
+    return (int)dispatch_grouped<1, 0>(m, k, n, pa, pb, out, variant, spec, s);
+}
+
+int wgrad(int groups, int rows, int m, int n, const int *row_offsets, const void *a_t, int a_fmt, const void *b_t, int b_fmt, int ld, void *out,
+          int out_type, const float *a_scale, const float *b_scale, int accumulate, int variant, void *stream)
+{
+    if (groups <= 0 || groups > kMaxGroups || rows <= 0 || m <= 0 || n <= 0 || !row_offsets || !a_t || !b_t || !out) return (int)hipErrorInvalidValue;
+    if (!fmt_ok(a_fmt) || !fmt_ok(b_fmt) || !wide_ok(out_type) || !wide_aligned(out, out_type)) return (int)hipErrorInvalidValue;
+    const int least = fp8gemm_grouped_ld(rows, groups);
+    if (least == 0 || ld < least || ld % kTokenRun != 0 || ld > (1 << 23)) return (int)hipErrorInvalidValue;
+    if (!aligned_to(a_t, 16) || !aligned_to(b_t, 16)) return (int)hipErrorInvalidValue;
+    const uint8_t *pa = static_cast<const uint8_t *>(a_t), *pb = static_cast<const uint8_t *>(b_t);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const GroupSpec spec = {row_offsets, groups, rows, a_scale, b_scale, 1, out_type, accumulate != 0};
+    (void)hipGetLastError();
+    if (a_fmt == FP8GEMM_E4M3 && b_fmt == FP8GEMM_E4M3) return (int)dispatch_wgrad<0, 0>(m, ld, n, pa, pb, out, variant, spec, s);
+    if (a_fmt == FP8GEMM_E5M2 && b_fmt == FP8GEMM_E5M2) return (int)dispatch_wgrad<1, 1>(m, ld, n, pa, pb, out, variant, spec, s);
+    if (a_fmt == FP8GEMM_E4M3) return (int)dispatch_wgrad<0, 1>(m, ld, n, pa, pb, out, variant, spec, s);
+    return (int)dispatch_wgrad<1, 0>(m, ld, n, pa, pb, out, variant, spec, s);
+}
+
+// ------------------------------------------------------------------ quantisation
+template <int TYPE, int FMT>
+hipError_t launch_quantize_rows(int rows, int cols, const void *x, size_t stride, int x_rows, const int *index, uint8_t *codes, float *scales, hipStream_t s)
+{
+    const size_t elem = TYPE == FP8GEMM_OUT_F32 ? 4 : 2;
+    const bool vec = cols % 8 == 0 && aligned_to(x, 16) && stride * elem % 16 == 0 && aligned_to(codes, 8);
+#define ROWS_KERNEL(WAVES, HELD)                                                                                                              \
+    hipLaunchKernelGGL((quantize_rows_kernel<TYPE, FMT, WAVES, HELD>), dim3((unsigned)((rows + 4 / WAVES - 1) / (4 / WAVES))), dim3(256), 0, s, \
+                       rows, cols, x, stride, x_rows, index, codes, scales)
+    // A wave to a row as long as a lane can hold its share; four waves for longer rows.
+    if (vec && cols <= 1024)
+        ROWS_KERNEL(1, 2);
+    else if (vec && cols <= 4096 && rows >= 1024)
+        ROWS_KERNEL(1, 8);
+    else if (vec && cols <= 4096)
+        ROWS_KERNEL(4, 2);
+    else if (vec && cols <= 16384)
+        ROWS_KERNEL(4, 8);
+    else
+        hipLaunchKernelGGL((quantize_rows_any_kernel<TYPE, FMT>), dim3((unsigned)rows), dim3(256), 0, s, cols, x, stride, x_rows, index, codes, scales);
+#undef ROWS_KERNEL
+    return hipGetLastError();
+}
+
+template <int TYPE, int FMT>
+hipError_t launch_quantize_columns(const GroupSpec &grp, int cols, const void *x, size_t stride, int x_rows, const int *index, uint8_t *codes, size_t ld,
+                                   float *scales, hipStream_t s)
+{
+    const size_t elem = TYPE == FP8GEMM_OUT_F32 ? 4 : 2;
+    const bool vec = cols % 8 == 0 && aligned_to(x, 16) && stride * elem % 16 == 0;
+    const long col_blocks = (cols + kColBlock - 1) / kColBlock;
+    const long grid = col_blocks * (grp.groups + 1);
+    if (grid > 0x7FFFFFFFL) return hipErrorInvalidValue;
+    if (vec)
+        hipLaunchKernelGGL((quantize_columns_kernel<TYPE, FMT, true>), dim3((unsigned)grid), dim3(256), 0, s, grp, cols, x, stride, x_rows, index, codes, ld,
+                           scales);
+    else
+        hipLaunchKernelGGL((quantize_columns_kernel<TYPE, FMT, false>), dim3((unsigned)grid), dim3(256), 0, s, grp, cols, x, stride, x_rows, index, codes, ld,
+                           scales);
+    return hipGetLastError();
+}
+
+bool quantize_source_ok(int rows, int cols, const void *x, int x_type, long long x_stride, int x_rows, const int *row_index, int fmt)
+{
+    if (rows <= 0 || cols <= 0 || x_rows <= 0 || !x || !wide_ok(x_type) || !fmt_ok(fmt) || x_stride < cols) return false;
+    return (row_index || rows <= x_rows) && wide_aligned(x, x_type);
+}
+
+// ------------------------------------------------------------------ 4-bit weights
+template <bool F16, int MODE, int RUN, int MT>
+struct W4KernelTag {};
+
+constexpr int kW4MaxLds = 160 * 1024;
+
+template <bool F16, int MODE, int RUN, int MT>
+hipError_t launch_w4_kernel(W4Args p, hipStream_t s)
+{
+    const int most_rows = std::min(p.rows, 16 * MT);
+    const int col_tiles = (p.n + 15) / 16;
+    // Waves along K until the grid has two workgroups for every CU, as long as each keeps a few ring stages of K.
+    int wk = 1;
+    while (wk < kW4Waves && (long)((col_tiles + kW4Waves / wk - 1) / (kW4Waves / wk)) * p.groups < 512 && p.k >= 4 * wk * kW4StageK) wk *= 2;
+    p.wk = wk;
+    const int wc = kW4Waves / wk;
+    // k staged at a time: all of it, or as much as leaves room for a second workgroup on the CU
+    const int unit = kW4StageK * wk;
+    int chunk = (p.k + unit - 1) / unit * unit;
+    while (chunk > unit && kW4RingBytes + w4_stage_bytes(most_rows, chunk, wc, RUN, p.zeros != nullptr) > kW4MaxLds / 2) {
+        chunk = (chunk / 2 + unit - 1) / unit * unit;
+    }
+    p.chunk = chunk;
+    const int parts = wk > 1 ? (wk - 1) * wc * MT * 1024 : 0;
+    const int lds = kW4RingBytes + std::max(w4_stage_bytes(most_rows, chunk, wc, RUN, p.zeros != nullptr), parts);
+    if (lds > kW4MaxLds) return hipErrorInvalidValue;
+    auto kernel = gemv_w4_kernel<F16, MODE, RUN, MT>;
+    hipError_t e = allow_lds<W4KernelTag<F16, MODE, RUN, MT>>(kernel, kW4MaxLds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((p.n + 16 * wc - 1) / (16 * wc)), (unsigned)p.groups), dim3(64 * kW4Waves), lds, s, p);
+    return hipGetLastError();
+}
+
+template <bool F16, int MODE, int RUN>
+hipError_t launch_w4_rows(const W4Args &p, hipStream_t s)
+{
+    // rows of x per pass over the weights; with experts, what an expert has on average
+    const int average = (p.rows + p.groups - 1) / p.groups;
+    if (p.rows <= 16 || average <= 8) return launch_w4_kernel<F16, MODE, RUN, 1>(p, s);
+    if (p.rows <= 32 || average <= 16) return launch_w4_kernel<F16, MODE, RUN, 2>(p, s);
+    return launch_w4_kernel<F16, MODE, RUN, 4>(p, s);
+}
+
+int gemv_w4(int groups, int m, int k, int n, const int *row_offsets, const void *x, int x_type, const float *x_scale, const void *w, int w_fmt, int run,
+            const void *w_scales, int scale_type, const void *w_zeros, void *y, int y_type, void *stream)
+{
+    if (groups <= 0 || groups > kMaxGroups || m <= 0 || k <= 0 || n <= 0 || run <= 0 || !x || !w || !w_scales || !y) return (int)hipErrorInvalidValue;
+    if (run % 32 != 0 || k % run != 0 || k > (1 << 23)) return (int)hipErrorInvalidValue;
+    if (w_fmt != FP8GEMM_W4_INT && w_fmt != FP8GEMM_W4_E2M1) return (int)hipErrorInvalidValue;
+    if (w_zeros && w_fmt != FP8GEMM_W4_INT) return (int)hipErrorInvalidValue;
+    if (x_type != FP8GEMM_T_BF16 && x_type != FP8GEMM_T_F16 && x_type != FP8GEMM_T_E4M3 && x_type != FP8GEMM_T_E5M2) return (int)hipErrorInvalidValue;
+    if (!wide_ok(scale_type) && scale_type != FP8GEMM_T_E8M0) return (int)hipErrorInvalidValue;
+    if (!wide_ok(y_type) || !wide_aligned(y, y_type) || !aligned_to(x, 16) || !aligned_to(w, 16)) return (int)hipErrorInvalidValue;
+    if (wide_ok(scale_type) && !wide_aligned(w_scales, scale_type)) return (int)hipErrorInvalidValue;
+    const W4Args p = {row_offsets, groups, m, k, n, x, x_type, x_scale, static_cast<const uint8_t *>(w), w_scales, scale_type,
+                      static_cast<const uint8_t *>(w_zeros), run, y, y_type, 0, 1};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    (void)hipGetLastError();
+    const bool f16 = x_type != FP8GEMM_T_BF16, long_runs = run % 128 == 0;
+    hipError_t e;
+    if (w_fmt == FP8GEMM_W4_INT) {
+        if (f16)
+            e = long_runs ? launch_w4_rows<true, kW4Int, 128>(p, s) : launch_w4_rows<true, kW4Int, 32>(p, s);
+        else
+            e = long_runs ? launch_w4_rows<false, kW4Int, 128>(p, s) : launch_w4_rows<false, kW4Int, 32>(p, s);
+    } else if (f16) {
+        e = long_runs ? launch_w4_rows<true, kW4Fp4, 128>(p, s) : launch_w4_rows<true, kW4Fp4, 32>(p, s);
+    } else {
+        e = long_runs ? launch_w4_rows<false, kW4Fp4, 128>(p, s) : launch_w4_rows<false, kW4Fp4, 32>(p, s);
+    }
+    return (int)e;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fp8gemm_grouped(int groups, int m, int k, int n, const int *row_offsets, const void *a, int a_fmt, const void *b, int b_fmt, void *out,
+                    int out_type, const float *a_scale, const float *b_scale, int b_scale_per_column, void *stream)
+{
+    return grouped(groups, m, k, n, row_offsets, a, a_fmt, b, b_fmt, out, out_type, a_scale, b_scale, b_scale_per_column, -1, stream);
+}
+
+int fp8gemm_grouped_tuned(int groups, int m, int k, int n, const int *row_offsets, const void *a, int a_fmt, const void *b, int b_fmt, void *out,
+                          int out_type, const float *a_scale, const float *b_scale, int b_scale_per_column, int variant, void *stream)
+{
+    return grouped(groups, m, k, n, row_offsets, a, a_fmt, b, b_fmt, out, out_type, a_scale, b_scale, b_scale_per_column, variant, stream);
+}
+
+int fp8gemm_grouped_ld(int rows, int groups)
+{
+    if (rows <= 0 || groups <= 0 || groups > kMaxGroups) return 0;
+    const long long ld = ((long long)rows + (long long)(kTokenRun - 1) * groups) / kTokenRun * kTokenRun;
+    return ld > (1 << 23) ? 0 : (int)ld;
+}
+
+int fp8gemm_grouped_wgrad(int groups, int rows, int m, int n, const int *row_offsets, const void *a_t, int a_fmt, const void *b_t, int b_fmt,
+                          int ld, void *out, int out_type, const float *a_scale, const float *b_scale, int accumulate, void *stream)
+{
+    return wgrad(groups, rows, m, n, row_offsets, a_t, a_fmt, b_t, b_fmt, ld, out, out_type, a_scale, b_scale, accumulate, -1, stream);
+}
+
+int fp8gemm_grouped_wgrad_tuned(int groups, int rows, int m, int n, const int *row_offsets, const void *a_t, int a_fmt, const void *b_t,
+                                int b_fmt, int ld, void *out, int out_type, const float *a_scale, const float *b_scale, int accumulate,
+                                int variant, void *stream)
+{
+    return wgrad(groups, rows, m, n, row_offsets, a_t, a_fmt, b_t, b_fmt, ld, out, out_type, a_scale, b_scale, accumulate, variant, stream);
+}
+
+int fp8gemm_quantize_rows(int rows, int cols, const void *x, int x_type, long long x_stride, int x_rows, const int *row_index, int fmt,
+                          void *codes, float *scales, void *stream)
+{
+    if (!codes || !scales || !quantize_source_ok(rows, cols, x, x_type, x_stride, x_rows, row_index, fmt)) return (int)hipErrorInvalidValue;
+    uint8_t *pc = static_cast<uint8_t *>(codes);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const size_t stride = (size_t)x_stride;
+    (void)hipGetLastError();
+#define QUANT(TYPE)                                                                                                       \
+    (fmt == FP8GEMM_E4M3 ? launch_quantize_rows<TYPE, 0>(rows, cols, x, stride, x_rows, row_index, pc, scales, s)         \
+                         : launch_quantize_rows<TYPE, 1>(rows, cols, x, stride, x_rows, row_index, pc, scales, s))
+    if (x_type == FP8GEMM_OUT_F32) return (int)QUANT(FP8GEMM_OUT_F32);
+    if (x_type == FP8GEMM_OUT_BF16) return (int)QUANT(FP8GEMM_OUT_BF16);
+    return (int)QUANT(FP8GEMM_OUT_F16);
+#undef QUANT
+}
+
+int fp8gemm_quantize_columns(int groups, int rows, int cols, const int *row_offsets, const void *x, int x_type, long long x_stride, int x_rows,
+                             const int *row_index, int fmt, void *codes_t, int ld, float *scales, void *stream)
+{
+    if (!codes_t || !scales || !row_offsets || !quantize_source_ok(rows, cols, x, x_type, x_stride, x_rows, row_index, fmt)) return (int)hipErrorInvalidValue;
+    const int least = fp8gemm_grouped_ld(rows, groups);
+    if (least == 0 || ld < least || ld % kTokenRun != 0 || ld > (1 << 23) || !aligned_to(codes_t, 16)) return (int)hipErrorInvalidValue;
+    uint8_t *pc = static_cast<uint8_t *>(codes_t);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const size_t stride = (size_t)x_stride;
+    const GroupSpec spec = {row_offsets, groups, rows, nullptr, nullptr, 0, 0, 0};
+    (void)hipGetLastError();
+#define QUANT(TYPE)                                                                                                         \
+    (fmt == FP8GEMM_E4M3 ? launch_quantize_columns<TYPE, 0>(spec, cols, x, stride, x_rows, row_index, pc, ld, scales, s)    \
+                         : launch_quantize_columns<TYPE, 1>(spec, cols, x, stride, x_rows, row_index, pc, ld, scales, s))
+    if (x_type == FP8GEMM_OUT_F32) return (int)QUANT(FP8GEMM_OUT_F32);
+    if (x_type == FP8GEMM_OUT_BF16) return (int)QUANT(FP8GEMM_OUT_BF16);
+    return (int)QUANT(FP8GEMM_OUT_F16);
+#undef QUANT
+}
+
+int fp8gemm_gemv_w4(int m, int k, int n, const void *x, int x_type, const float *x_scale, const void *w, int w_fmt, int run, const void *w_scales,
+                    int scale_type, const void *w_zeros, void *y, int y_type, void *stream)
+{
+    return gemv_w4(1, m, k, n, nullptr, x, x_type, x_scale, w, w_fmt, run, w_scales, scale_type, w_zeros, y, y_type, stream);
+}
+
+int fp8gemm_grouped_w4(int groups, int m, int k, int n, const int *row_offsets, const void *x, int x_type, const float *x_scale, const void *w,
+                       int w_fmt, int run, const void *w_scales, int scale_type, const void *w_zeros, void *y, int y_type, void *stream)
+{
+    if (!row_offsets) return (int)hipErrorInvalidValue;
+    return gemv_w4(groups, m, k, n, row_offsets, x, x_type, x_scale, w, w_fmt, run, w_scales, scale_type, w_zeros, y, y_type, stream);
+}
+
+}  // extern "C"

@@ -35,7 +35,7 @@ extern template hipError_t dispatch_bell<1, 0>(int, int, int, const uint8_t *, c
 extern template hipError_t dispatch_bell<1, 1>(int, int, int, const uint8_t *, const uint8_t *, float *, const BellSpec &, Workspace &, hipStream_t);
 
 namespace {
-constexpr int kVersion = 103;
+constexpr int kVersion = 104;
 // What the work lists and the planner's constants are laid out for: MI355X as one partition,
 // 256 CUs in 8 XCDs of 32, workgroups handed to the XCDs round robin (id mod 8).  On another
 // partition mode every result is still right (the work list only decides who computes what);

@@ -29,6 +29,10 @@
 // turns the epilogue into 128-bit stores.
 //
 // LDS layout, swizzle and the K-permutation freedom are described in kernel_tile.h.
+//
+// The products grouped by expert (GROUPED, GroupSpec in group_table.h) run the same pipeline: only the
+// work list, which is laid out on the device from the row offsets, where a tile's operands and results
+// lie, and the scales of the epilogue differ.
 // Requirements checked by the host: K % 16 == 0 (rows start 16-byte aligned and a
 // 16-byte chunk never straddles the end of a row), K < 2^23, 16-byte aligned a and b.
 #ifndef FP8GEMM_KERNEL_PTILE_H
@@ -36,6 +40,7 @@
 
 #include <type_traits>
 
+#include "group_table.h"
 #include "kernel_tile.h"
 
 // s_waitcnt on the LDS/scalar counter only
@@ -121,8 +126,10 @@ constexpr bool ptile_sums_slices_in_kernel = S::BM * S::BN <= 128 * 128;
 // bf16 / fp16); without it C receives the bare fp32 sums and `spec` is ignored.  BSTREAM: B is
 // loaded with the non-temporal hint (for a C with a single row of tiles, where every byte of B
 // is read by exactly one workgroup).  BELL: A is sparse in blocked-ELL form (`bell`).  NOPF: without
-// the L2 prefetch (see NPF below).
-template <class S, int AF, int BF, bool KOVER, bool EX, bool BSTREAM, bool BELL, bool NOPF>
+// the L2 prefetch (see NPF below).  GROUPED: the products grouped by expert (`grp`): kGroupedRows cuts the
+// rows of A and C among the groups and gives each its own B, kGroupedK cuts K (the tokens; K is then the
+// row stride of A and B) and gives each group its own C; bulk, tail, rounds, tiles_m come from the group table.
+template <class S, int AF, int BF, bool KOVER, bool EX, bool BSTREAM, bool BELL, bool NOPF, int GROUPED = kNotGrouped>
 __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
                                                 const uint8_t *__restrict__ A,
                                                 const uint8_t *__restrict__ B,
@@ -131,8 +138,9 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
                                                 int *__restrict__ counters,
                                                 int tiles_m, int tiles_n, int GM, int CB,
                                                 int bulk, int tail, int nsplit,
-                                                int rounds, int rotate_and_skew, OutSpec spec, BellSpec bell)
+                                                int rounds, int rotate_and_skew, OutSpec spec, BellSpec bell, GroupSpec grp = GroupSpec{})
 {
+    static_assert(GROUPED == kNotGrouped || (!BELL && !EX && NOPF), "the grouped forms have their own epilogue and no prefetch");
     static_assert(!BELL || !BSTREAM, "the blocked-ELL form shares B between tile rows");
     // Small blocks (tiles of fewer than 128 rows): a 128-byte K tile spans several stored blocks, so
     // where a chunk of B lies depends on which `bell.sub` bytes of the K tile (one stored block, or the
@@ -190,6 +198,18 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
     // write C directly.
     const int xcd = blockIdx.x & 7;
     const int slot = blockIdx.x >> 3;
+    // Grouped: the tiles of group 0 come first, then those of group 1, ..; inside a group the numbering is
+    // the one above.  The table in LDS holds every group's first tile number and the row offsets.
+    LDS_AS int *tab_tile = (LDS_AS int *)(lds + S::PTILE_LDS_BYTES + kGroupTableOffset + 2 * (BM + BN) * 4);
+    LDS_AS int *tab_row = tab_tile + kMaxGroups + 1;
+    if constexpr (GROUPED != kNotGrouped) {
+        const int total = build_group_table<GROUPED == kGroupedRows ? BM : BK>(grp, GROUPED == kGroupedRows ? 0 : tiles_m, tiles_n, tab_tile, tab_row);
+        bulk = total / 256 * 256;
+        tail = total - bulk;
+        rounds = (total + 255) / 256;
+    }
+    int g_row0 = 0, g_row_end = 0, g_id = 0;      // grouped: first row, end of the group's rows, group of the planned item
+    int g_kt = 0;                                  // kGroupedK: K tiles of the planned item that hold tokens
     const int bulk_rounds = bulk >> 8;
     const int tail_items = tail * nsplit;
 
@@ -220,6 +240,28 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
             if (nsplit > 1) ws_slot = slice * tail + t;
         }
         int row, col;
+        if constexpr (GROUPED != kNotGrouped) {
+            g_id = group_of_tile(grp.groups, tab_tile, g);
+            g -= __builtin_amdgcn_readfirstlane((int)tab_tile[g_id]);
+            const int first = __builtin_amdgcn_readfirstlane((int)tab_row[g_id]), end = __builtin_amdgcn_readfirstlane((int)tab_row[g_id + 1]);
+            const int tm_g = GROUPED == kGroupedRows ? (end - first + BM - 1) / BM : tiles_m;
+            tile_of_number(g, tm_g, tiles_n, tm_g < 4 ? tm_g : 4, tiles_n, row, col);
+            tn = __builtin_amdgcn_readfirstlane(col);
+            tm = __builtin_amdgcn_readfirstlane(row);
+            if constexpr (GROUPED == kGroupedRows) {
+                g_row0 = first + tm * BM;
+                g_row_end = end;
+                kt0 = 0;
+                T = KT;
+            } else {
+                // the rows of a group start at its place in the padded token axis and fill whole K tiles
+                // (the 16x16x128 schedule needs two: missing ones read as zeros, see issue_load)
+                kt0 = first;
+                g_kt = end - first;
+                T = S::MF16 && g_kt < 2 ? 2 : g_kt;
+            }
+            return true;
+        }
         tile_of_number(g, tiles_m, tiles_n, GM, CB, row, col);
         // (the divisions may run on the vector unit; every lane holds the same values)
         tn = __builtin_amdgcn_readfirstlane(col);
@@ -323,19 +365,40 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
         }
         bell_chunk = chunk;
     };
+    int g_set = 1;                                 // grouped: which set of scales the planned item uses
     auto plan_loads = [&](int tile_m, int tile_n, int kt0, int count, int item) __attribute__((always_inline)) {
-        const int m0 = tile_m * BM, n0 = tile_n * BN;
-        const int rows_a = M - m0 < BM ? M - m0 : BM;
+        const int m0 = GROUPED == kGroupedRows ? g_row0 : tile_m * BM, n0 = tile_n * BN;
+        const int m_end = GROUPED == kGroupedRows ? g_row_end : M;
+        const int rows_a = m_end - m0 < BM ? m_end - m0 : BM;
         const int rows_b = N - n0 < BN ? N - n0 : BN;
+        const size_t b_row0 = GROUPED == kGroupedRows ? (size_t)g_id * N + n0 : (size_t)n0;
         rsA = make_buffer_resource(A + (size_t)m0 * K, (unsigned long long)rows_a * (unsigned long long)K);
-        rsB = make_buffer_resource(B + (size_t)n0 * KB, (unsigned long long)rows_b * (unsigned long long)KB);
+        rsB = make_buffer_resource(B + b_row0 * KB, (unsigned long long)rows_b * (unsigned long long)KB);
+        if constexpr (GROUPED != kNotGrouped) {
+            // The scales of the tile's rows and columns travel with its first operand loads, straight into LDS
+            // (rows and columns past the end take the last one's: their results are not stored).  Two sets,
+            // alternating: the epilogue of the tile before may still be reading its own.
+            g_set ^= 1;
+            const uint32_t at = lds_base + (uint32_t)(S::PTILE_LDS_BYTES + kGroupTableOffset + g_set * (BM + BN) * 4 + wave * 256);
+            const int q = wave * 64 + lane;
+            if (grp.a_scale && wave * 64 < BM) {
+                const int row = m0 + (q < rows_a ? q : rows_a - 1);
+                const float *p = grp.a_scale + (GROUPED == kGroupedRows ? (size_t)row : (size_t)g_id * M + row);
+                global_load_lds_b32(reinterpret_cast<const uint8_t *>(p), at);
+            }
+            if (grp.b_scale && wave * 64 < BN) {
+                const int col = n0 + (q < rows_b ? q : rows_b - 1);
+                const float *p = grp.b_scale + (grp.b_per_column ? (size_t)g_id * N + col : (size_t)g_id);
+                global_load_lds_b32(reinterpret_cast<const uint8_t *>(p), at + (uint32_t)(BM * 4));
+            }
+        }
         if constexpr (BELL) bell_row = bell.cols + (size_t)(m0 / bell.block) * bell.ell_cols;
         kt_base = kt0;
         kt_count = count;
         const unsigned key = rotate == 1 ? (unsigned)tile_n : (unsigned)item;   // item: (round, XCD)
         // (the division runs on the vector unit; the result is the same in every lane)
-        kt_rot = rotate == 0 ? 0 : __builtin_amdgcn_readfirstlane((int)(((key * 2654435761u) >> 8) % (unsigned)count));
-        plan_prefetch(tile_m, tile_n, items_in_xcd);
+        kt_rot = rotate == 0 || (GROUPED == kGroupedK && count == 0) ? 0 : __builtin_amdgcn_readfirstlane((int)(((key * 2654435761u) >> 8) % (unsigned)count));
+        if constexpr (GROUPED == kNotGrouped) plan_prefetch(tile_m, tile_n, items_in_xcd);
         if constexpr (BELL) bell_fetch(0);
     };
     // load number j (0 .. LOADS-1) of step `ktile` of the planned item's K walk into ring slot `stage`
@@ -385,6 +448,13 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
                                      bell_pad ? 0u : bell_koff);
                 return;
             }
+        }
+        if constexpr (GROUPED == kGroupedK && S::MF16) {
+            // a K tile past the group's tokens (the next group's): outside an empty extent, reads zeros
+            v4i rs = j < S::A_LOADS ? rsA : rsB;
+            rs[2] = kk < g_kt ? rs[2] : 0;
+            buffer_load_lds_b128(rs, j < S::A_LOADS ? ldsA + sbase + (uint32_t)(j * RPI * BK) : ldsB + sbase + (uint32_t)((j - S::A_LOADS) * RPI * BK), voff, koff);
+            return;
         }
         if (j < S::A_LOADS)
             buffer_load_lds_b128(rsA, ldsA + sbase + (uint32_t)(j * RPI * BK), voff, koff);
@@ -451,7 +521,9 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
             }
             continue;
         }
-        const int m0 = tile_m * BM, n0 = tile_n * BN;
+        const int m0 = GROUPED == kGroupedRows ? g_row0 : tile_m * BM, n0 = tile_n * BN;
+        const int m_end = GROUPED == kGroupedRows ? g_row_end : M;
+        const int c_group = g_id, c_set = g_set;       // (the planned item changes before the epilogue)
 
         // accumulators: TM x TN blocks of 32 x 32 (16 registers each), or twice as many
         // blocks of 16 x 16 each way (4 registers each); 256 registers per lane either way
@@ -696,7 +768,8 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
         // (the scratch takes bare fp32 sums; scale and output type are applied where C is written)
         const bool to_ws = ws_slot >= 0;
         void *__restrict__ tile_base = to_ws ? static_cast<void *>(ws) : C;
-        const size_t tile_origin = to_ws ? (size_t)ws_slot * (size_t)(BM * BN) : (size_t)m0 * (size_t)N + n0;
+        const size_t tile_origin = to_ws ? (size_t)ws_slot * (size_t)(BM * BN)
+                                         : (size_t)m0 * (size_t)N + n0 + (GROUPED == kGroupedK ? (size_t)c_group * M * N : 0);
         const size_t ldo = to_ws ? (size_t)BN : (size_t)N;
         // (the epilogue arithmetic -- scales, beta * C, largest magnitude -- only where C itself is
         // written, and only in the kernels compiled for it)
@@ -751,6 +824,38 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
                 const int lrow0 = wrow0 - m0 + i * 32 + rl;          // inside the tile
                 const int lcol_ = wcol0 - n0 + c0 + cl * 4;
                 const size_t first = tile_origin + (size_t)lrow0 * ldo + lcol_;
+                if constexpr (GROUPED != kNotGrouped) {
+                    // The same order of LDS reads and stores as below; most tiles are ragged, so every store is
+                    // guarded, four columns at a time where rows of C keep that alignment.
+                    const LDS_AS float *sa = (const LDS_AS float *)(lds + S::PTILE_LDS_BYTES + kGroupTableOffset + c_set * (BM + BN) * 4);
+                    const LDS_AS float *sb = sa + BM;
+                    v4f buf[NR], fb = {1.0f, 1.0f, 1.0f, 1.0f};
+                    float fa[NR];
+                    if (grp.b_scale) fb = *reinterpret_cast<const LDS_AS v4f *>(sb + lcol_);
+#pragma unroll
+                    for (int u = 0; u < NR; ++u) {
+                        buf[u] = *reinterpret_cast<const v4f *>(stg + (u * RPI_ST + rl) * ROWB + cl * 16);
+                        fa[u] = grp.a_scale ? sa[lrow0 + u * RPI_ST] : 1.0f;
+                    }
+                    if constexpr (ST + 1 < NSTEP) stage_strip(std::integral_constant<int, ST + 1>{});
+                    __builtin_amdgcn_sched_barrier(0);
+                    const bool quads = N % 4 == 0 && reinterpret_cast<uintptr_t>(C) % 16 == 0;
+#pragma unroll
+                    for (int u = 0; u < NR; ++u) {
+                        const size_t index = first + (size_t)(u * RPI_ST) * ldo;
+                        if (m0 + lrow0 + u * RPI_ST >= m_end || n0 + lcol_ >= N) continue;
+                        v4f y = {buf[u][0] * fa[u] * fb[0], buf[u][1] * fa[u] * fb[1], buf[u][2] * fa[u] * fb[2], buf[u][3] * fa[u] * fb[3]};
+                        if (quads) {
+                            if (grp.accumulate) y += load_in4(C, index, grp.type);
+                            store_out4_stream(C, index, y, grp.type);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (n0 + lcol_ + e < N) store_out(C, index + e, grp.accumulate ? y[e] + load_in(C, index + e, grp.type) : y[e], grp.type);
+                        }
+                    }
+                    return;
+                }
                 if (full) {
                     // All reads of the strip go out back to back, then the next strip is staged
                     // (the LDS serves one wave's instructions in order, so those writes land after
@@ -924,6 +1029,19 @@ __global__ __launch_bounds__(S::THREADS) void gemm_ptile_bell_kernel(int M, int 
     // (tiles of fewer than 128 rows serve small blocks, whose stored rows need not be whole K tiles)
     gemm_ptile_body<S, AF, BF, (S::BM < 128), false, false, true, false>(M, K, N, A, B, C, ws, counters, tiles_m, tiles_n, GM, CB, bulk, tail,
                                                           nsplit, rounds, rotate_and_skew, plain, bell);
+}
+
+// Products grouped by expert (GROUPED: kGroupedRows or kGroupedK).
+template <class S, int AF, int BF, bool KOVER, bool BSTREAM, int GROUPED>
+__global__ __launch_bounds__(S::THREADS) void gemm_ptile_grouped_kernel(int M, int K, int N,
+                                                                         const uint8_t *__restrict__ A,
+                                                                         const uint8_t *__restrict__ B,
+                                                                         void *__restrict__ C,
+                                                                         int tiles_m, int tiles_n, int rotate, GroupSpec grp)
+{
+    const OutSpec plain = {1.0f, nullptr, nullptr, FP8GEMM_DEV_OUT_F32, 0.0f, nullptr, FP8GEMM_DEV_OUT_F32, nullptr, nullptr, nullptr};
+    gemm_ptile_body<S, AF, BF, KOVER, false, BSTREAM, false, true, GROUPED>(M, K, N, A, B, C, nullptr, nullptr, tiles_m, tiles_n, 4, tiles_n, 0, 0,
+                                                                            1, 0, rotate, plain, BellSpec{nullptr, 0, 0, 0, 0}, grp);
 }
 
 #endif  // FP8GEMM_KERNEL_PTILE_H

@@ -11,6 +11,7 @@
 
 #include "device_common.h"
 #include "fp8gemm.h"
+#include "group_table.h"
 
 namespace fp8gemm_detail {
 
@@ -102,6 +103,16 @@ hipError_t dispatch(int m, int k, int n, const uint8_t *a, const uint8_t *b, voi
 template <int AF, int BF>
 hipError_t dispatch_bell(int m, int kell, int n, const uint8_t *values, const uint8_t *b, float *out, const BellSpec &bell,
                          Workspace &wsp, hipStream_t stream);
+
+// Products grouped by expert: tile shapes by the numbers above, or the kernel for any shape.
+constexpr int kGroupedDirect = 0;
+int plan_grouped(int m, int k, int n, int groups);
+int plan_wgrad(int m, int n, int rows, int groups);
+// variant < 0: the plan's choice.  grouped: rows of A and C cut among the groups; wgrad: K (the tokens, row stride ld).
+template <int AF, int BF>
+hipError_t dispatch_grouped(int m, int k, int n, const uint8_t *a, const uint8_t *b, void *out, int variant, const GroupSpec &grp, hipStream_t stream);
+template <int AF, int BF>
+hipError_t dispatch_wgrad(int m, int ld, int n, const uint8_t *a_t, const uint8_t *b_t, void *out, int variant, const GroupSpec &grp, hipStream_t stream);
 
 }  // namespace fp8gemm_detail
 

@@ -1,0 +1,90 @@
+"""Refusals of the entry points for layers with experts: before anything touches the GPU."""
+import ctypes
+
+import pytest
+
+INVALID = 1      # hipErrorInvalidValue
+P = ctypes.c_void_p(0x1000)
+ODD = ctypes.c_void_p(0x1001)
+
+
+def call(fn, good, **change):
+    args = dict(good)
+    args.update(change)
+    return fn(*args.values())
+
+
+def refused(fn, good, changes):
+    for change in changes:
+        assert call(fn, good, **change) == INVALID, change
+
+
+GROUPED = dict(groups=4, m=100, k=256, n=128, row_offsets=P, a=P, a_fmt=0, b=P, b_fmt=0, out=P, out_type=0, a_scale=None, b_scale=None, per_column=0, stream=None)
+WGRAD = dict(groups=4, rows=100, m=64, n=64, row_offsets=P, a_t=P, a_fmt=0, b_t=P, b_fmt=0, ld=512, out=P, out_type=0, a_scale=None, b_scale=None, accumulate=0, stream=None)
+QROWS = dict(rows=10, cols=64, x=P, x_type=1, x_stride=64, x_rows=10, row_index=None, fmt=0, codes=P, scales=P, stream=None)
+QCOLS = dict(groups=4, rows=100, cols=64, row_offsets=P, x=P, x_type=1, x_stride=64, x_rows=100, row_index=None, fmt=0, codes_t=P, ld=512, scales=P, stream=None)
+W4 = dict(m=1, k=256, n=64, x=P, x_type=1, x_scale=None, w=P, w_fmt=0, run=128, w_scales=P, scale_type=2, w_zeros=None, y=P, y_type=1, stream=None)
+
+
+def test_grouped(pkg):
+    changes = [dict(groups=0), dict(groups=1025), dict(groups=-1), dict(m=0), dict(k=0), dict(n=-3), dict(row_offsets=None), dict(a=None), dict(b=None), dict(out=None), dict(a_fmt=2), dict(b_fmt=-1),
+               dict(out_type=3), dict(out_type=-1), dict(out=ODD), dict(out=ODD, out_type=1)]
+    refused(pkg.lib().fp8gemm_grouped, GROUPED, changes)
+    tuned = dict(GROUPED)
+    del tuned["stream"]
+    tuned.update(variant=6, stream=None)
+    # shapes that a kernel cannot run, and numbers that name none
+    refused(pkg.lib().fp8gemm_grouped_tuned, tuned, [dict(variant=1), dict(variant=14), dict(variant=99), dict(variant=13, k=128), dict(variant=6, k=100), dict(variant=15, a=ODD), dict(variant=5, k=(1 << 23) + 16)])
+
+
+def test_wgrad(pkg):
+    changes = [dict(groups=0), dict(groups=1025), dict(rows=0), dict(m=0), dict(n=0), dict(row_offsets=None), dict(a_t=None), dict(b_t=None), dict(out=None), dict(a_fmt=5), dict(b_fmt=5), dict(out_type=7),
+               dict(ld=384), dict(ld=513), dict(ld=(1 << 23) + 128), dict(rows=1000), dict(a_t=ODD), dict(b_t=ODD), dict(out=ODD)]
+    refused(pkg.lib().fp8gemm_grouped_wgrad, WGRAD, changes)
+    tuned = dict(WGRAD)
+    del tuned["stream"]
+    tuned.update(variant=6, stream=None)
+    refused(pkg.lib().fp8gemm_grouped_wgrad_tuned, tuned, [dict(variant=0), dict(variant=5), dict(variant=15)])
+
+
+def test_quantize(pkg):
+    common = [dict(rows=0), dict(cols=0), dict(x=None), dict(x_type=3), dict(x_type=-1), dict(x_stride=63), dict(x_rows=0), dict(fmt=2), dict(scales=None), dict(x=ODD), dict(x_rows=9)]
+    refused(pkg.lib().fp8gemm_quantize_rows, QROWS, common + [dict(codes=None)])
+    refused(pkg.lib().fp8gemm_quantize_columns, QCOLS, common + [dict(codes_t=None), dict(codes_t=ODD), dict(row_offsets=None), dict(groups=0), dict(groups=2000), dict(ld=256), dict(ld=500), dict(rows=1 << 24, x_rows=1 << 24)])
+
+
+def test_padded_length(pkg):
+    """Whole runs of 128 for every expert, whatever the cut; 0 for what is no length."""
+    ld = pkg.lib().fp8gemm_grouped_ld
+    for rows, groups in ((1, 1), (128, 1), (129, 1), (100, 4), (1, 1024), (4096, 8), (5, 7)):
+        worst = 128 * (min(groups, rows) - 1) + -(-(rows - min(groups, rows) + 1) // 128) * 128      # as many experts as possible with one row
+        assert ld(rows, groups) % 128 == 0 and ld(rows, groups) >= worst
+    assert ld(0, 1) == 0 and ld(1, 0) == 0 and ld(1, 1025) == 0 and ld(1 << 24, 1) == 0
+
+
+def test_w4(pkg):
+    changes = [dict(m=0), dict(k=0), dict(n=0), dict(run=0), dict(run=48), dict(run=96), dict(run=16), dict(x=None), dict(w=None), dict(w_scales=None), dict(y=None), dict(w_fmt=2), dict(w_fmt=1, w_zeros=P),
+               dict(x_type=0), dict(x_type=5), dict(scale_type=3), dict(scale_type=6), dict(y_type=3), dict(x=ODD), dict(w=ODD), dict(y=ODD), dict(w_scales=ODD), dict(k=1 << 24)]
+    refused(pkg.lib().fp8gemm_gemv_w4, W4, changes)
+    grouped = dict(groups=4, m=1, k=256, n=64, row_offsets=P)
+    grouped.update({key: W4[key] for key in list(W4)[3:]})
+    refused(pkg.lib().fp8gemm_grouped_w4, grouped, changes + [dict(row_offsets=None), dict(groups=0), dict(groups=1025)])
+
+
+def test_python_checks_need_no_gpu(pkg):
+    """Tensors that are not on a GPU, or do not fit, are refused before a call is made."""
+    import torch
+    a, b = torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(2, 16, 32, dtype=torch.uint8)
+    off = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.gemm_grouped(a, b, off, a_fmt=0, b_fmt=0)
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.gemm_grouped_wgrad(a, b[0], off, 8, a_fmt=0, b_fmt=0)
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.quantize_rows(torch.zeros(4, 64))
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.quantize_rows(torch.zeros(4, 64).t())
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.quantize_columns(torch.zeros(4, 64), off)
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.gemv_w4(torch.zeros(1, 64, dtype=torch.bfloat16), torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2), 32)

@@ -1,0 +1,170 @@
+"""Wide numbers to fp8 codes with power-of-two scales, by rows and transposed by expert: codes and scales are exact."""
+import zlib
+
+import numpy as np
+import pytest
+import torch
+
+from expert_util import F8, TOP, offsets_of, places, quantized
+
+pytestmark = pytest.mark.gpu
+
+WIDE = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def generator(*key):
+    return torch.Generator(device="cuda").manual_seed(zlib.crc32(repr(key).encode()))
+
+
+def wide(gen, rows, cols, dtype):
+    x = torch.randn((rows, cols), generator=gen, device="cuda") * torch.exp2(torch.randint(-9, 4, (rows, 1), generator=gen, device="cuda").float())
+    return x.to(dtype)
+
+
+def same(got, want):
+    got = got.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+
+
+@pytest.mark.parametrize("dtype", WIDE)
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 8), (5, 7), (1, 4096), (9, 1032), (1500, 4096), (1030, 1024), (4, 4104), (3, 16384), (2, 16392), (7, 4095), (2, 20000)])
+def test_rows(pkg, dtype, fmt, rows, cols):
+    """Every kernel: a wave to a row, four waves, any length; lengths that are not whole pieces."""
+    x = wide(generator("rows", rows, cols), rows, cols, dtype)
+    v, s = quantized(x, fmt, 1)
+    got, scales = pkg.quantize_rows(x, fmt)
+    assert got.dtype == F8[fmt] and torch.equal(scales.double(), s)
+    same(got, v)
+
+
+@pytest.mark.parametrize("dtype", WIDE)
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("cols", [72, 75, 1040, 4100])
+def test_rows_hard_numbers(pkg, dtype, fmt, cols):
+    """Zeros, infinities, NaNs, the type's largest and smallest numbers, maxima on and beside a power of two times the
+    largest code."""
+    gen = generator("hard", cols)
+    x = wide(gen, 12, cols, dtype)
+    big, small = torch.finfo(dtype).max, torch.finfo(dtype).smallest_normal
+    x[0] = 0
+    x[1] = -0.0
+    x[2, 3], x[2, 5], x[2, cols - 1] = float("inf"), float("-inf"), float("nan")
+    x[3] = float("nan")
+    x[4] = float("inf")
+    x[5, cols // 2] = big
+    x[6] = 0
+    x[6, 1] = -big
+    x[7] = 0
+    x[7, cols - 2] = small
+    for r, m in ((8, 0.875), (9, 0.875 * (1 + torch.finfo(dtype).eps)), (10, 0.875 * (1 - torch.finfo(dtype).eps)), (11, 1.0)):
+        x[r] = (x[r].float().clamp(-0.5, 0.5)).to(dtype)
+        x[r, r] = m
+    v, s = quantized(x, fmt, 1)
+    got, scales = pkg.quantize_rows(x, fmt)
+    assert torch.equal(scales.double(), s)
+    same(got, v)
+    nan = torch.isnan(x)
+    assert (got.view(torch.uint8)[nan] == 0x7F).all()
+    assert (got.view(torch.uint8)[1] == 0x80).all()
+    assert (got[4].float() == TOP[fmt]).all()
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+def test_rows_codes_equal_the_host_codec(pkg, fmt):
+    """Every rounding: all midpoints and their neighbours, scale 1, against the library's host conversion."""
+    from conftest import finite_codes
+    v = np.sort(pkg.decode(finite_codes(fmt), fmt))
+    mid = (v[1:].astype(np.float64) + v[:-1]) / 2
+    pts = np.concatenate([v, mid, np.nextafter(mid.astype(np.float32), np.float32(1e9)), np.nextafter(mid.astype(np.float32), np.float32(-1e9))]).astype(np.float32)
+    pts = pts[np.abs(pts) <= TOP[fmt]]
+    pts = np.concatenate([pts, np.full(-pts.size % 8, TOP[fmt], np.float32)])
+    got, scales = pkg.quantize_rows(torch.from_numpy(pts[None]).cuda(), fmt)
+    assert float(scales[0]) == 1.0
+    assert np.array_equal(got.view(torch.uint8).cpu().numpy()[0], pkg.encode(pts, fmt))
+
+
+@pytest.mark.parametrize("cols", [64, 65, 2048, 4096])
+def test_rows_gathered_and_strided(pkg, cols):
+    gen = generator("gather", cols)
+    store = wide(gen, 40, cols + 24, torch.bfloat16)
+    index = torch.randint(0, 40, (1200,), generator=gen, dtype=torch.int32, device="cuda")
+    index[3], index[7], index[11] = -1, 40, 2 ** 31 - 1
+    for shift in (0, 8, 3):                                  # rows that start on 16 bytes, and that do not
+        x = store[:, shift:shift + cols]
+        got, scales = pkg.quantize_rows(x, 0, row_index=index)
+        there = (index >= 0) & (index < 40)
+        rows = torch.where(there[:, None], x[index.clamp(0, 39).long()], torch.zeros((), dtype=x.dtype, device="cuda"))
+        v, s = quantized(rows, 0, 1)
+        assert torch.equal(scales.double(), s)
+        same(got, v)
+
+
+def check_columns(pkg, x, counts, fmt, index=None, first=0):
+    off = offsets_of(counts, first)
+    got, scales = pkg.quantize_columns(x, off, fmt, row_index=index)
+    rows = x if index is None else torch.where(((index >= 0) & (index < x.shape[0]))[:, None], x[index.clamp(0, x.shape[0] - 1).long()], torch.zeros((), dtype=x.dtype, device="cuda"))
+    at, cs, used = places(off.tolist(), rows.shape[0])
+    want = torch.zeros(got.shape, dtype=torch.float64, device="cuda")
+    for g, (p, c) in enumerate(zip(at, cs)):
+        v, s = quantized(rows[int(off[g]):int(off[g]) + c], fmt, 0) if c else (None, torch.ones(x.shape[1], dtype=torch.float64, device="cuda"))
+        assert torch.equal(scales[g].double(), s)
+        if c:
+            want[:, p:p + c] = v.t()
+    same(got, want)
+
+
+@pytest.mark.parametrize("dtype", WIDE)
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("cols", [1, 64, 72, 200, 75])
+@pytest.mark.parametrize("counts", [[1], [0, 5, 0, 131, 128, 0], [300, 1, 0, 1000], [i % 4 for i in range(67)]])
+def test_columns(pkg, dtype, fmt, cols, counts):
+    gen = generator("columns", cols, counts)
+    check_columns(pkg, wide(gen, sum(counts), cols, dtype), counts, fmt)
+
+
+@pytest.mark.parametrize("dtype", WIDE)
+@pytest.mark.parametrize("cols", [64, 75])
+def test_columns_hard_numbers(pkg, dtype, cols):
+    gen = generator("hard columns", cols)
+    x = wide(gen, 150, cols, dtype)
+    big = torch.finfo(dtype).max
+    x[:, 0] = 0
+    x[100, 1], x[101, 2], x[102, 3] = float("nan"), float("inf"), float("-inf")
+    x[:, 4] = float("nan")
+    x[5, 5] = big
+    for fmt in (0, 1):
+        check_columns(pkg, x, [20, 0, 100, 30], fmt)
+
+
+def test_columns_gathered_strided_and_rows_outside(pkg):
+    gen = generator("columns gather")
+    store = wide(gen, 50, 160, torch.float16)
+    index = torch.randint(0, 50, (333,), generator=gen, dtype=torch.int32, device="cuda")
+    index[0], index[300] = -5, 50
+    for shift in (0, 8, 5):
+        x = store[:, shift:shift + 136]
+        check_columns(pkg, x, [100, 0, 233], 0, index=index)
+        check_columns(pkg, x, [10, 3, 20], 1, first=7)               # rows in front of the first and behind the last expert
+
+
+def test_calls_captured_and_replayed(pkg):
+    gen = generator("graph")
+    x = wide(gen, 256, 512, torch.bfloat16)
+    off = offsets_of([100, 0, 156])
+    codes, scales = pkg.quantize_rows(x)
+    codes_t, scales_t = pkg.quantize_columns(x, off)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pkg.quantize_rows(x, codes=codes, scales=scales)
+        pkg.quantize_columns(x, off, codes=codes_t, scales=scales_t)
+    for cut in ([256, 0, 0], [3, 250, 3], [0, 0, 0]):
+        x.copy_(wide(gen, 256, 512, torch.bfloat16))
+        off.copy_(offsets_of(cut))
+        graph.replay()
+        torch.cuda.synchronize()
+        v, s = pkg.quantize_rows(x)
+        vt, st = pkg.quantize_columns(x, off)
+        assert torch.equal(v.view(torch.uint8), codes.view(torch.uint8)) and torch.equal(s, scales)
+        assert torch.equal(vt.view(torch.uint8), codes_t.view(torch.uint8)) and torch.equal(st, scales_t)
