@@ -416,45 +416,48 @@ def sddmm(row_offsets, col_idx, vec_length, lhs, rhs, l_fmt=None, r_fmt=None, ou
 W4_INT, W4_E2M1 = 0, 1
 T_F32, T_BF16, T_F16, T_E4M3, T_E5M2, T_E8M0 = 0, 1, 2, 3, 4, 5
 
+# (A serving step makes hundreds of these calls on matrices of a few rows, where the host decides the time: the
+# checks below are written to cost a few microseconds.)
+
 
 def _wide_code(dtype):
     import torch
-    codes = {torch.float32: OUT_F32, torch.bfloat16: OUT_BF16, torch.float16: OUT_F16}
-    if dtype not in codes:
-        raise Fp8GemmError("expected float32, bfloat16 or float16, got %s" % dtype)
-    return codes[dtype]
+    if dtype is torch.bfloat16:
+        return OUT_BF16
+    if dtype is torch.float32:
+        return OUT_F32
+    if dtype is torch.float16:
+        return OUT_F16
+    raise Fp8GemmError("expected float32, bfloat16 or float16, got %s" % dtype)
 
 
-def _same_device(*tensors):
+def _device_of(first, *others):
     """The device of the operands, which have to share one."""
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) != 1 or not next(iter(devices)).type == "cuda":
-        raise Fp8GemmError("operands must live in the memory of one device")
-    return devices.pop()
+    device = first.device
+    if device.type != "cuda":
+        raise Fp8GemmError("operands must live in device memory")
+    for t in others:
+        if t is not None and t.device != device:
+            raise Fp8GemmError("operands must live in the memory of one device")
+    return device
 
 
-class _on_device:
-    """Makes the operands' device current for a launch (the library launches on the current one); the
+def _launch(fn, device, stream, *args):
+    """fn(*args, stream) with the operands' device current (the library launches on the current one); the
     stream defaults to that device's current stream."""
-
-    def __init__(self, device, stream):
-        import torch
-        self._guard = torch.cuda.device(device)
-        self._stream = stream
-
-    def __enter__(self):
-        import torch
-        self._guard.__enter__()
-        return ctypes.c_void_p((self._stream or torch.cuda.current_stream()).cuda_stream)
-
-    def __exit__(self, *exc):
-        return self._guard.__exit__(*exc)
-
-
-def _contiguous(what, *tensors):
-    for t in tensors:
-        if t is not None and not t.is_contiguous():
-            raise Fp8GemmError("%s must be contiguous" % what)
+    import torch
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _launch(fn, device, stream, *args)
+    if stream is None:
+        handle = torch._C._cuda_getCurrentRawStream(device.index)
+    else:
+        if stream.device != device:
+            raise Fp8GemmError("the stream belongs to another device than the operands")
+        handle = stream.cuda_stream
+    code = fn(*args, handle)
+    if code != 0:
+        check(code)
 
 
 def _floats(t, count, what):
@@ -462,23 +465,23 @@ def _floats(t, count, what):
     import torch
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.numel() != count or not t.is_contiguous():
+    if t.dtype is not torch.float32 or t.numel() != count or not t.is_contiguous():
         raise Fp8GemmError("%s: expected %d contiguous float32 elements" % (what, count))
     return t.data_ptr()
 
 
 def _offsets(t):
-    if t.dim() != 1 or t.numel() < 2:
+    if t.dim() != 1 or t.shape[0] < 2:
         raise Fp8GemmError("row_offsets holds one more element than there are experts")
-    return _dev_ints(t), t.numel() - 1
+    return _dev_ints(t), t.shape[0] - 1
 
 
 def _output(out, shape, dtype, device):
     import torch
     if out is None:
         return torch.empty(shape, dtype=dtype or torch.float32, device=device)
-    if tuple(out.shape) != tuple(shape) or not out.is_contiguous() or (dtype is not None and out.dtype != dtype):
-        raise Fp8GemmError("out must be a contiguous %s tensor of the wanted type" % (tuple(shape),))
+    if tuple(out.shape) != shape or not out.is_contiguous() or (dtype is not None and out.dtype != dtype):
+        raise Fp8GemmError("out must be a contiguous %s tensor of the wanted type" % (shape,))
     return out
 
 
@@ -487,23 +490,37 @@ def grouped_ld(rows, groups):
     return lib().fp8gemm_grouped_ld(rows, groups)
 
 
+def _wide_matrix(x, row_index):
+    """rows of the result, columns, type code, row stride of a matrix to be quantised."""
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise Fp8GemmError("x must be a matrix whose rows are contiguous")
+    x_rows, cols = x.shape
+    stride = x.stride(0) if x_rows > 1 else cols
+    if stride < cols:
+        raise Fp8GemmError("the rows of x overlap")
+    return (x_rows if row_index is None else row_index.numel()), x_rows, cols, _wide_code(x.dtype), stride
+
+
+def _fp8_dtype(fmt):
+    import torch
+    if fmt == E4M3:
+        return torch.float8_e4m3fn
+    if fmt == E5M2:
+        return torch.float8_e5m2
+    raise Fp8GemmError("fmt is E4M3 or E5M2")
+
+
 def quantize_rows(x, fmt=E4M3, row_index=None, codes=None, scales=None, stream=None):
     """(codes, scales) of the rows of x (float32 / bfloat16 / float16, unit column stride), or of the rows
     row_index (int32) names (an index outside x: a row of zeros): codes (rows, cols) float8, scales (rows,)
     float32 powers of two, x ~ codes * scales[:, None].  Through fp8gemm_quantize_rows."""
     import torch
-    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
-        raise Fp8GemmError("x must be a matrix whose rows are contiguous")
-    rows = x.shape[0] if row_index is None else row_index.numel()
-    dtype = {E4M3: torch.float8_e4m3fn, E5M2: torch.float8_e5m2}[fmt]
-    device = _same_device(x, row_index, codes, scales)
-    codes = _output(codes, (rows, x.shape[1]), dtype, device)
+    rows, x_rows, cols, x_type, stride = _wide_matrix(x, row_index)
+    device = _device_of(x, row_index, codes, scales)
+    codes = _output(codes, (rows, cols), _fp8_dtype(fmt), device)
     scales = _output(scales, (rows,), torch.float32, device)
-    stride = x.stride(0) if x.shape[0] > 1 else x.shape[1]
-    with _on_device(device, stream) as s:
-        check(lib().fp8gemm_quantize_rows(rows, x.shape[1], x.data_ptr(), _wide_code(x.dtype), stride, x.shape[0],
-                                          None if row_index is None else _dev_ints(row_index), fmt, codes.data_ptr(),
-                                          scales.data_ptr(), s))
+    _launch(lib().fp8gemm_quantize_rows, device, stream, rows, cols, x.data_ptr(), x_type, stride, x_rows,
+            None if row_index is None else _dev_ints(row_index), fmt, codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
@@ -512,19 +529,14 @@ def quantize_columns(x, row_offsets, fmt=E4M3, row_index=None, codes=None, scale
     every expert's tokens in whole runs of 128 columns with zeros behind them, scales (groups, cols).
     row_index as in quantize_rows.  Through fp8gemm_quantize_columns."""
     import torch
-    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
-        raise Fp8GemmError("x must be a matrix whose rows are contiguous")
+    rows, x_rows, cols, x_type, stride = _wide_matrix(x, row_index)
+    device = _device_of(x, row_offsets, row_index, codes, scales)
     offs, groups = _offsets(row_offsets)
-    rows, cols = x.shape[0] if row_index is None else row_index.numel(), x.shape[1]
-    dtype = {E4M3: torch.float8_e4m3fn, E5M2: torch.float8_e5m2}[fmt]
-    device = _same_device(x, row_offsets, row_index, codes, scales)
-    codes = _output(codes, (cols, grouped_ld(rows, groups)), dtype, device)
+    ld = grouped_ld(rows, groups)
+    codes = _output(codes, (cols, ld), _fp8_dtype(fmt), device)
     scales = _output(scales, (groups, cols), torch.float32, device)
-    stride = x.stride(0) if x.shape[0] > 1 else cols
-    with _on_device(device, stream) as s:
-        check(lib().fp8gemm_quantize_columns(groups, rows, cols, offs, x.data_ptr(), _wide_code(x.dtype), stride, x.shape[0],
-                                             None if row_index is None else _dev_ints(row_index), fmt, codes.data_ptr(),
-                                             codes.shape[1], scales.data_ptr(), s))
+    _launch(lib().fp8gemm_quantize_columns, device, stream, groups, rows, cols, offs, x.data_ptr(), x_type, stride, x_rows,
+            None if row_index is None else _dev_ints(row_index), fmt, codes.data_ptr(), ld, scales.data_ptr())
     return codes, scales
 
 
@@ -533,20 +545,20 @@ def gemm_grouped(a, b, row_offsets, a_scale=None, b_scale=None, out_dtype=None, 
     """out[i] = a_scale[i] * b_scale[g] * (a[i] . b[g]^T) for the rows i of every expert g: a (m, k), b (groups, n, k)
     codes, row_offsets (groups + 1,) int32, a_scale (m,), b_scale (groups, n) or (groups,) float32 or None.
     Rows outside the experts are left as they are (uninitialised when out is None).  Through fp8gemm_grouped."""
-    _contiguous("operands", a, b)
+    device = _device_of(a, b, row_offsets, a_scale, b_scale, out)
     if a.dim() != 2 or b.dim() != 3 or a.shape[1] != b.shape[2]:
         raise Fp8GemmError("a (m, k) and b (groups, n, k) do not fit")
+    if not (a.is_contiguous() and b.is_contiguous()):
+        raise Fp8GemmError("operands must be contiguous")
     offs, groups = _offsets(row_offsets)
     if b.shape[0] != groups:
         raise Fp8GemmError("row_offsets is for %d experts, b holds %d" % (groups, b.shape[0]))
     (m, k), n = a.shape, b.shape[1]
-    device = _same_device(a, b, row_offsets, a_scale, b_scale, out)
     out = _output(out, (m, n), out_dtype, device)
     per_column = b_scale is not None and b_scale.dim() == 2
-    sa, sb = _floats(a_scale, m, "a_scale"), _floats(b_scale, groups * n if per_column else groups, "b_scale")
-    with _on_device(device, stream) as s:
-        check(lib().fp8gemm_grouped_tuned(groups, m, k, n, offs, a.data_ptr(), _fmt_of(a, a_fmt), b.data_ptr(), _fmt_of(b, b_fmt),
-                                          out.data_ptr(), _wide_code(out.dtype), sa, sb, int(per_column), variant, s))
+    _launch(lib().fp8gemm_grouped_tuned, device, stream, groups, m, k, n, offs, a.data_ptr(), _fmt_of(a, a_fmt), b.data_ptr(),
+            _fmt_of(b, b_fmt), out.data_ptr(), _wide_code(out.dtype), _floats(a_scale, m, "a_scale"),
+            _floats(b_scale, groups * n if per_column else groups, "b_scale"), int(per_column), variant)
     return out
 
 
@@ -555,20 +567,19 @@ def gemm_grouped_wgrad(a_t, b_t, row_offsets, rows, a_scale=None, b_scale=None, 
     """out[g] = a_scale[g][:, None] * b_scale[g] * (a_t . b_t^T over the tokens of expert g): a_t (m, ld), b_t (n, ld) codes
     as quantize_columns lays them out for `rows` rows, a_scale (groups, m), b_scale (groups, n) float32 or None;
     out (groups, m, n), added to what it holds if accumulate.  Through fp8gemm_grouped_wgrad."""
-    _contiguous("operands", a_t, b_t)
+    device = _device_of(a_t, b_t, row_offsets, a_scale, b_scale, out)
     if a_t.dim() != 2 or b_t.dim() != 2 or a_t.shape[1] != b_t.shape[1]:
         raise Fp8GemmError("a_t (m, ld) and b_t (n, ld) do not fit")
-    offs, groups = _offsets(row_offsets)
-    (m, ld), n = a_t.shape, b_t.shape[0]
-    device = _same_device(a_t, b_t, row_offsets, a_scale, b_scale, out)
+    if not (a_t.is_contiguous() and b_t.is_contiguous()):
+        raise Fp8GemmError("operands must be contiguous")
     if accumulate and out is None:
         raise Fp8GemmError("accumulate needs the tensor to add to")
+    offs, groups = _offsets(row_offsets)
+    (m, ld), n = a_t.shape, b_t.shape[0]
     out = _output(out, (groups, m, n), out_dtype, device)
-    sa, sb = _floats(a_scale, groups * m, "a_scale"), _floats(b_scale, groups * n, "b_scale")
-    with _on_device(device, stream) as s:
-        check(lib().fp8gemm_grouped_wgrad_tuned(groups, rows, m, n, offs, a_t.data_ptr(), _fmt_of(a_t, a_fmt), b_t.data_ptr(),
-                                                _fmt_of(b_t, b_fmt), ld, out.data_ptr(), _wide_code(out.dtype), sa, sb,
-                                                int(bool(accumulate)), variant, s))
+    _launch(lib().fp8gemm_grouped_wgrad_tuned, device, stream, groups, rows, m, n, offs, a_t.data_ptr(), _fmt_of(a_t, a_fmt),
+            b_t.data_ptr(), _fmt_of(b_t, b_fmt), ld, out.data_ptr(), _wide_code(out.dtype), _floats(a_scale, groups * m, "a_scale"),
+            _floats(b_scale, groups * n, "b_scale"), int(bool(accumulate)), variant)
     return out
 
 
@@ -579,40 +590,37 @@ def gemv_w4(x, w, scales, run, w_fmt=W4_INT, zeros=None, x_scale=None, row_offse
     uint8 or None, x_scale (m,) float32 or None.  With row_offsets (groups + 1,) the rows of x are sorted by expert and
     w, scales, zeros have a leading axis of experts.  Through fp8gemm_gemv_w4 / fp8gemm_grouped_w4."""
     import torch
-    _contiguous("operands", x, w, scales, zeros)
-    if x.dim() != 2:
-        raise Fp8GemmError("x must be a matrix")
+    device = _device_of(x, w, scales, zeros, x_scale, row_offsets, out)
+    if x.dim() != 2 or not (x.is_contiguous() and w.is_contiguous()):
+        raise Fp8GemmError("x must be a matrix, operands contiguous")
     m, k = x.shape
-    lead = ()
-    offs, groups = None, 1
-    if row_offsets is not None:
+    if row_offsets is None:
+        offs, groups, lead = None, 1, ()
+    else:
         offs, groups = _offsets(row_offsets)
         lead = (groups,)
-    if w.dim() != 2 + len(lead) or w.dtype != torch.uint8 or tuple(w.shape[:-2]) != lead or 2 * w.shape[-1] != k:
-        raise Fp8GemmError("w must hold %s x n x k/2 bytes" % (groups,))
+    if w.dtype is not torch.uint8 or w.dim() != 2 + len(lead) or w.shape[:-2] != lead or 2 * w.shape[-1] != k:
+        raise Fp8GemmError("w must hold %d x n x k/2 bytes" % groups)
     n = w.shape[-2]
     if run <= 0 or k % run:
         raise Fp8GemmError("run must divide k")
-    for t, what in ((scales, "scales"), (zeros, "zeros")):
-        if t is not None and tuple(t.shape) != lead + (n, k // run):
-            raise Fp8GemmError("%s must have the shape %s" % (what, lead + (n, k // run)))
-    if zeros is not None and zeros.dtype != torch.uint8:
-        raise Fp8GemmError("zeros are bytes")
-    scale_type = T_E8M0 if scales.dtype == torch.uint8 else _wide_code(scales.dtype)
-    if x.dtype in (torch.bfloat16, torch.float16):
-        x_type = T_BF16 if x.dtype == torch.bfloat16 else T_F16
+    shape = lead + (n, k // run)
+    if scales.shape != shape or not scales.is_contiguous():
+        raise Fp8GemmError("scales must have the shape %s" % (shape,))
+    if zeros is not None and (zeros.shape != shape or not zeros.is_contiguous() or zeros.dtype is not torch.uint8):
+        raise Fp8GemmError("zeros must be bytes of the shape %s" % (shape,))
+    scale_type = T_E8M0 if scales.dtype is torch.uint8 else _wide_code(scales.dtype)
+    if x.dtype is torch.bfloat16:
+        x_type = T_BF16
+    elif x.dtype is torch.float16:
+        x_type = T_F16
     else:
         x_type = T_E4M3 if _fmt_of(x, x_fmt) == E4M3 else T_E5M2
-    device = _same_device(x, w, scales, zeros, x_scale, row_offsets, out)
     out = _output(out, (m, n), out_dtype, device)
-    sx = _floats(x_scale, m, "x_scale")
-    L, pz = lib(), None if zeros is None else zeros.data_ptr()
-    with _on_device(device, stream) as s:
-        if offs is None:
-            code = L.fp8gemm_gemv_w4(m, k, n, x.data_ptr(), x_type, sx, w.data_ptr(), w_fmt, run, scales.data_ptr(), scale_type, pz,
-                                     out.data_ptr(), _wide_code(out.dtype), s)
-        else:
-            code = L.fp8gemm_grouped_w4(groups, m, k, n, offs, x.data_ptr(), x_type, sx, w.data_ptr(), w_fmt, run, scales.data_ptr(),
-                                        scale_type, pz, out.data_ptr(), _wide_code(out.dtype), s)
-        check(code)
+    args = (m, k, n, x.data_ptr(), x_type, _floats(x_scale, m, "x_scale"), w.data_ptr(), w_fmt, run, scales.data_ptr(), scale_type,
+            None if zeros is None else zeros.data_ptr(), out.data_ptr(), _wide_code(out.dtype))
+    if offs is None:
+        _launch(lib().fp8gemm_gemv_w4, device, stream, *args)
+    else:
+        _launch(lib().fp8gemm_grouped_w4, device, stream, groups, m, k, n, offs, *args[3:])
     return out

@@ -6,6 +6,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "dispatch.h"
 #include "kernel_quantize.h"
@@ -23,20 +24,59 @@ extern template hipError_t dispatch_wgrad<1, 0>(int, int, int, const uint8_t *, 
 extern template hipError_t dispatch_wgrad<1, 1>(int, int, int, const uint8_t *, const uint8_t *, void *, int, const GroupSpec &, hipStream_t);
 
 // ------------------------------------------------------------------ planning
-// The cut of the rows is known on the device only: the tile is chosen by the average rows of an expert.
+// Cost model in microseconds, as plan_tile's (fp8gemm.hip): a round of whole tiles is k_tiles * per_k_tile + per_item, a
+// round that is not full costs its K tiles times idle + (1 - idle) * (share of its tiles), and no launch is faster than
+// its bytes at stream_rate.  Fitted to 120 cuts (1 to 64 experts, 1 to 4096 rows each, k 256 to 8192, n 512 to 8192): the
+// pick takes 2 % longer than the best of nine measured shapes on average.  The cut itself is known on the device
+// only: an expert is taken to have the average of rows, and half a tile of rows in a tile that is not full.
+struct GroupedCost {
+    int variant, bm, bn, per_cu;
+    bool overhang;                                            // compiled for a K that is not a multiple of 128
+    double per_k_tile, per_item, stream_rate, idle;           // us, us, bytes per us
+};
+constexpr GroupedCost kGroupedCosts[] = {
+    {13, 256, 256, 1, true, 1.44, 7.6, 4.65e6, 0.60},
+    {14, 192, 256, 1, false, 1.18, 6.2, 4.9e6, 0.64},
+    // two workgroups on a CU: 128 x 128 tiles, with the non-temporal hint on B and without; 64 x 128 with it
+    {17, 128, 128, 2, false, 1.20, 2.2, 8.4e6, 0.44},
+    {18, 128, 128, 2, true, 1.07, 2.25, 5.1e6, 0.30},
+    {19, 64, 128, 2, true, 1.06, 1.4, 1e9, 0.23},
+    // one workgroup on a CU, a deeper ring: no more tiles than CUs
+    {15, 64, 128, 1, false, 0.466, 2.2, 6.2e6, 0.63},
+};
+
 int plan_grouped(int m, int k, int n, int groups)
 {
-    const int average = (m + groups - 1) / groups;
-    if (average <= 64) return 15;
-    if (average <= 256 || !p2h_ok(k, 1)) return 6;
-    return 13;
+    const double kt = (k + 127) / 128;
+    const int busy = m < groups ? m : groups;
+    const double average = (double)m / busy;
+    const double bytes = (double)busy * n * k + (double)m * k + 2.0 * m * n;
+    int pick = 18;
+    double best = 1e30;
+    for (const GroupedCost &c : kGroupedCosts) {
+        if (k % 128 != 0 && !c.overhang) continue;
+        if ((c.variant == 13 || c.variant == 14) && !p2h_ok(k, 1)) continue;
+        const double rows_of_tiles = groups == 1 ? (double)((m + c.bm - 1) / c.bm) : busy * std::max(1.0, average / c.bm + 0.5);
+        const double rounds = rows_of_tiles * ((n + c.bn - 1) / c.bn) / (256.0 * c.per_cu);
+        const double whole = std::floor(rounds), rest = rounds - whole;
+        double cost = whole * (kt * c.per_k_tile + c.per_item);
+        if (rest > 1e-9) cost += kt * c.per_k_tile * (c.idle + (1.0 - c.idle) * rest) + c.per_item;
+        cost = std::max(cost, bytes / c.stream_rate);
+        if (cost < best) {
+            best = cost;
+            pick = c.variant;
+        }
+    }
+    return pick;
 }
 
-int plan_wgrad(int m, int n, int rows, int groups)
+// The weight gradient: the 256 x 256 tile on the 16x16x128 MFMA once an expert has some four K tiles of tokens, below
+// that the 128 x 128 tile with two workgroups on a CU, whose epilogues overlap (bf16 output, us, 128 x 128 / 256 x 256: 16 experts
+// of 2048 x 1024, 128 tokens each 24.3 / 27.1, 512 33.5 / 35.1, 2048 85.7 / 79.7; 4 of 8192 x 4096, 256 tokens 98.9 / 101.7, 512
+// 122.8 / 115.4, 4096 524 / 396; 128 x 256 and 192 x 256 tiles lie behind one of the two everywhere).
+int plan_wgrad(int rows, int groups)
 {
-    (void)rows;
-    const long tiles = (long)((m + 255) / 256) * ((n + 255) / 256) * groups;
-    return tiles >= 256 ? 13 : 6;
+    return rows / groups < 512 ? 18 : 13;
 }
 
 }  // namespace fp8gemm_detail

@@ -129,7 +129,7 @@ constexpr bool ptile_sums_slices_in_kernel = S::BM * S::BN <= 128 * 128;
 // the L2 prefetch (see NPF below).  GROUPED: the products grouped by expert (`grp`): kGroupedRows cuts the
 // rows of A and C among the groups and gives each its own B, kGroupedK cuts K (the tokens; K is then the
 // row stride of A and B) and gives each group its own C; bulk, tail, rounds, tiles_m come from the group table.
-template <class S, int AF, int BF, bool KOVER, bool EX, bool BSTREAM, bool BELL, bool NOPF, int GROUPED = kNotGrouped>
+template <class S, int AF, int BF, bool KOVER, bool EX, bool BSTREAM, bool BELL, bool NOPF, int GROUPED = kNotGrouped, int PER_CU = 1>
 __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
                                                 const uint8_t *__restrict__ A,
                                                 const uint8_t *__restrict__ B,
@@ -140,7 +140,7 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
                                                 int bulk, int tail, int nsplit,
                                                 int rounds, int rotate_and_skew, OutSpec spec, BellSpec bell, GroupSpec grp = GroupSpec{})
 {
-    static_assert(GROUPED == kNotGrouped || (!BELL && !EX && NOPF), "the grouped forms have their own epilogue and no prefetch");
+    static_assert(GROUPED == kNotGrouped || (!BELL && !EX), "the grouped forms have their own epilogue");
     static_assert(!BELL || !BSTREAM, "the blocked-ELL form shares B between tile rows");
     // Small blocks (tiles of fewer than 128 rows): a 128-byte K tile spans several stored blocks, so
     // where a chunk of B lies depends on which `bell.sub` bytes of the K tile (one stored block, or the
@@ -198,19 +198,21 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
     // write C directly.
     const int xcd = blockIdx.x & 7;
     const int slot = blockIdx.x >> 3;
+    constexpr int ROUND = 256 * PER_CU;            // workgroups that run at the same time
     // Grouped: the tiles of group 0 come first, then those of group 1, ..; inside a group the numbering is
     // the one above.  The table in LDS holds every group's first tile number and the row offsets.
     LDS_AS int *tab_tile = (LDS_AS int *)(lds + S::PTILE_LDS_BYTES + kGroupTableOffset + 2 * (BM + BN) * 4);
-    LDS_AS int *tab_row = tab_tile + kMaxGroups + 1;
+    LDS_AS int *tab_row = tab_tile + grp.groups + 1;
     if constexpr (GROUPED != kNotGrouped) {
         const int total = build_group_table<GROUPED == kGroupedRows ? BM : BK>(grp, GROUPED == kGroupedRows ? 0 : tiles_m, tiles_n, tab_tile, tab_row);
-        bulk = total / 256 * 256;
+        bulk = total / ROUND * ROUND;
         tail = total - bulk;
-        rounds = (total + 255) / 256;
+        rounds = (total + ROUND - 1) / ROUND;
     }
     int g_row0 = 0, g_row_end = 0, g_id = 0;      // grouped: first row, end of the group's rows, group of the planned item
+    int g_strip = 1;                               // tile rows of a strip of the planned item's group
     int g_kt = 0;                                  // kGroupedK: K tiles of the planned item that hold tokens
-    const int bulk_rounds = bulk >> 8;
+    const int bulk_rounds = bulk / ROUND;
     const int tail_items = tail * nsplit;
 
     // item of round r: tile, slice, K-tile range [kt0, kt0 + T), scratch slot (-1: writes C);
@@ -221,13 +223,13 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
         int g, slice = 0;
         ws_slot = -1;
         if (r < bulk_rounds) {
-            if (slot >= 32) return false;
-            items_in_xcd = 32;
-            g = r * 256 + xcd * 32 + slot;
+            if (slot >= ROUND / 8) return false;
+            items_in_xcd = ROUND / 8;
+            g = r * ROUND + xcd * (ROUND / 8) + slot;
         } else {
-            const int first = (r - bulk_rounds) * 256;
+            const int first = (r - bulk_rounds) * ROUND;
             int count = tail_items - first;
-            count = count > 256 ? 256 : count;
+            count = count > ROUND ? ROUND : count;
             if (count <= 0) return false;
             const int per_xcd = (count + 7) >> 3;
             items_in_xcd = per_xcd;
@@ -245,7 +247,8 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
             g -= __builtin_amdgcn_readfirstlane((int)tab_tile[g_id]);
             const int first = __builtin_amdgcn_readfirstlane((int)tab_row[g_id]), end = __builtin_amdgcn_readfirstlane((int)tab_row[g_id + 1]);
             const int tm_g = GROUPED == kGroupedRows ? (end - first + BM - 1) / BM : tiles_m;
-            tile_of_number(g, tm_g, tiles_n, tm_g < 4 ? tm_g : 4, tiles_n, row, col);
+            g_strip = tm_g < 4 ? tm_g : 4;
+            tile_of_number(g, tm_g, tiles_n, g_strip, tiles_n, row, col);
             tn = __builtin_amdgcn_readfirstlane(col);
             tm = __builtin_amdgcn_readfirstlane(row);
             if constexpr (GROUPED == kGroupedRows) {
@@ -308,6 +311,23 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
     const uint8_t *pf_ptr = A;
     auto plan_prefetch = [&](int tile_m_, int tile_n_, int items_in_xcd) __attribute__((always_inline)) {
         const int q = wave * 64 + lane;                      // 0 .. 255: line number inside this workgroup's share
+        if constexpr (GROUPED != kNotGrouped) {
+            // (a group's tiles start anywhere in the XCD's window: the shares go by the tile's place in its strip)
+            const int m0 = GROUPED == kGroupedRows ? g_row0 : tile_m_ * BM, m_end = GROUPED == kGroupedRows ? g_row_end : M;
+            const int nb = (BN + g_strip - 1) / g_strip, na = (BM + 7) / 8;
+            const uint8_t *p = A + (size_t)m0 * K;
+            if (q < nb) {
+                int row = tile_n_ * BN + (tile_m_ % g_strip) * nb + q;
+                row = row < N ? row : N - 1;
+                p = B + ((GROUPED == kGroupedRows ? (size_t)g_id * N : 0) + row) * KB;
+            } else if (q - nb < na) {
+                int row = m0 + (tile_n_ % 8) * na + (q - nb);
+                row = row < m_end ? row : m_end - 1;
+                p = A + (size_t)row * K;
+            }
+            pf_ptr = p;
+            return;
+        }
         int a_parts = items_in_xcd / GM;
         a_parts = a_parts > 8 ? 8 : (a_parts < 1 ? 1 : a_parts);
         const int nb = (BN + GM - 1) / GM, na = (BM + a_parts - 1) / a_parts;
@@ -398,7 +418,7 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
         const unsigned key = rotate == 1 ? (unsigned)tile_n : (unsigned)item;   // item: (round, XCD)
         // (the division runs on the vector unit; the result is the same in every lane)
         kt_rot = rotate == 0 || (GROUPED == kGroupedK && count == 0) ? 0 : __builtin_amdgcn_readfirstlane((int)(((key * 2654435761u) >> 8) % (unsigned)count));
-        if constexpr (GROUPED == kNotGrouped) plan_prefetch(tile_m, tile_n, items_in_xcd);
+        plan_prefetch(tile_m, tile_n, items_in_xcd);
         if constexpr (BELL) bell_fetch(0);
     };
     // load number j (0 .. LOADS-1) of step `ktile` of the planned item's K walk into ring slot `stage`
@@ -476,7 +496,13 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
         kk += kt_rot;
         kk = kk >= kt_count ? kk - kt_count : kk;
         // (K is a multiple of 16: the last, overhanging K tile still starts inside the row)
-        const uint32_t koff = (uint32_t)__builtin_amdgcn_readfirstlane((kt_base + kk) * BK);
+        int at = kt_base + kk;
+        if constexpr (GROUPED == kGroupedK) {
+            // (the 16x16x128 schedule walks two K tiles of a group that has one or none: this load, unlike those of the
+            // operands, goes by no buffer extent, so it stays on the group's own K tiles, or on the first one)
+            at = g_kt == 0 ? 0 : (kk < g_kt ? at : kt_base + g_kt - 1);
+        }
+        const uint32_t koff = (uint32_t)__builtin_amdgcn_readfirstlane(at * BK);
         global_load_lds_b32(pf_ptr + koff, lds_base + (uint32_t)S::PTILE_LDS_BYTES);
     };
     // Prefetch instructions that close a batch of loads, and how many K tiles they run ahead of
@@ -781,6 +807,8 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
         const bool full = to_ws || ((m0 + BM <= M) && (n0 + BN <= N) && (N % 4 == 0) &&
                                     (reinterpret_cast<uintptr_t>(C) % 16 == 0) &&
                                     (!EX || !spec.c || reinterpret_cast<uintptr_t>(spec.c) % 16 == 0));
+        // (grouped: a tile without an overhang)
+        const bool g_whole = m0 + BM <= m_end && n0 + BN <= N;
         {
             // Each wave transposes its results through a private strip of LDS (the part of
             // the ring the next tile's first loads do not use, plus the LDS above the ring)
@@ -825,12 +853,29 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
                 const int lcol_ = wcol0 - n0 + c0 + cl * 4;
                 const size_t first = tile_origin + (size_t)lrow0 * ldo + lcol_;
                 if constexpr (GROUPED != kNotGrouped) {
-                    // The same order of LDS reads and stores as below; most tiles are ragged, so every store is
-                    // guarded, four columns at a time where rows of C keep that alignment.
+                    // The same order of LDS reads and stores as below.
                     const LDS_AS float *sa = (const LDS_AS float *)(lds + S::PTILE_LDS_BYTES + kGroupTableOffset + c_set * (BM + BN) * 4);
                     const LDS_AS float *sb = sa + BM;
+                    const bool quads = N % 4 == 0 && reinterpret_cast<uintptr_t>(C) % 16 == 0;
                     v4f buf[NR], fb = {1.0f, 1.0f, 1.0f, 1.0f};
                     float fa[NR];
+                    if (!quads || grp.accumulate) {
+                        // single elements, or C read back: a few rows at a time
+#pragma unroll 1
+                        for (int r0 = 0; r0 < 32; r0 += RPI_ST) {
+                            const v4f v = *reinterpret_cast<const v4f *>(stg + (r0 + rl) * ROWB + cl * 16);
+                            const float a = grp.a_scale ? sa[lrow0 + r0] : 1.0f;
+                            const size_t index = first + (size_t)r0 * ldo;
+                            if (m0 + lrow0 + r0 < m_end)
+                                for (int e = 0; e < 4; ++e)
+                                    if (n0 + lcol_ + e < N) {
+                                        const float y = v[e] * a * (grp.b_scale ? sb[lcol_ + e] : 1.0f);
+                                        store_out(C, index + e, grp.accumulate ? y + load_in(C, index + e, grp.type) : y, grp.type);
+                                    }
+                        }
+                        if constexpr (ST + 1 < NSTEP) stage_strip(std::integral_constant<int, ST + 1>{});
+                        return;
+                    }
                     if (grp.b_scale) fb = *reinterpret_cast<const LDS_AS v4f *>(sb + lcol_);
 #pragma unroll
                     for (int u = 0; u < NR; ++u) {
@@ -839,20 +884,19 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
                     }
                     if constexpr (ST + 1 < NSTEP) stage_strip(std::integral_constant<int, ST + 1>{});
                     __builtin_amdgcn_sched_barrier(0);
-                    const bool quads = N % 4 == 0 && reinterpret_cast<uintptr_t>(C) % 16 == 0;
+                    if (g_whole) {
+#pragma unroll
+                        for (int u = 0; u < NR; ++u) {
+                            const v4f y = {buf[u][0] * fa[u] * fb[0], buf[u][1] * fa[u] * fb[1], buf[u][2] * fa[u] * fb[2], buf[u][3] * fa[u] * fb[3]};
+                            store_out4_stream(C, first + (size_t)(u * RPI_ST) * ldo, y, grp.type);
+                        }
+                        return;
+                    }
+                    // a ragged tile: the same with every store guarded (columns go in whole fours)
 #pragma unroll
                     for (int u = 0; u < NR; ++u) {
-                        const size_t index = first + (size_t)(u * RPI_ST) * ldo;
-                        if (m0 + lrow0 + u * RPI_ST >= m_end || n0 + lcol_ >= N) continue;
-                        v4f y = {buf[u][0] * fa[u] * fb[0], buf[u][1] * fa[u] * fb[1], buf[u][2] * fa[u] * fb[2], buf[u][3] * fa[u] * fb[3]};
-                        if (quads) {
-                            if (grp.accumulate) y += load_in4(C, index, grp.type);
-                            store_out4_stream(C, index, y, grp.type);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (n0 + lcol_ + e < N) store_out(C, index + e, grp.accumulate ? y[e] + load_in(C, index + e, grp.type) : y[e], grp.type);
-                        }
+                        const v4f y = {buf[u][0] * fa[u] * fb[0], buf[u][1] * fa[u] * fb[1], buf[u][2] * fa[u] * fb[2], buf[u][3] * fa[u] * fb[3]};
+                        if (m0 + lrow0 + u * RPI_ST < m_end && n0 + lcol_ < N) store_out4_stream(C, first + (size_t)(u * RPI_ST) * ldo, y, grp.type);
                     }
                     return;
                 }
@@ -1032,15 +1076,15 @@ __global__ __launch_bounds__(S::THREADS) void gemm_ptile_bell_kernel(int M, int 
 }
 
 // Products grouped by expert (GROUPED: kGroupedRows or kGroupedK).
-template <class S, int AF, int BF, bool KOVER, bool BSTREAM, int GROUPED>
-__global__ __launch_bounds__(S::THREADS) void gemm_ptile_grouped_kernel(int M, int K, int N,
+template <class S, int AF, int BF, bool KOVER, bool BSTREAM, bool NOPF, int GROUPED, int PER_CU>
+__global__ __launch_bounds__(S::THREADS, PER_CU) void gemm_ptile_grouped_kernel(int M, int K, int N,
                                                                          const uint8_t *__restrict__ A,
                                                                          const uint8_t *__restrict__ B,
                                                                          void *__restrict__ C,
                                                                          int tiles_m, int tiles_n, int rotate, GroupSpec grp)
 {
     const OutSpec plain = {1.0f, nullptr, nullptr, FP8GEMM_DEV_OUT_F32, 0.0f, nullptr, FP8GEMM_DEV_OUT_F32, nullptr, nullptr, nullptr};
-    gemm_ptile_body<S, AF, BF, KOVER, false, BSTREAM, false, true, GROUPED>(M, K, N, A, B, C, nullptr, nullptr, tiles_m, tiles_n, 4, tiles_n, 0, 0,
+    gemm_ptile_body<S, AF, BF, KOVER, false, BSTREAM, false, NOPF, GROUPED, PER_CU>(M, K, N, A, B, C, nullptr, nullptr, tiles_m, tiles_n, 4, tiles_n, 0, 0,
                                                                             1, 0, rotate, plain, BellSpec{nullptr, 0, 0, 0, 0}, grp);
 }
 

@@ -32,9 +32,9 @@ def test_grouped(pkg):
     refused(pkg.lib().fp8gemm_grouped, GROUPED, changes)
     tuned = dict(GROUPED)
     del tuned["stream"]
-    tuned.update(variant=6, stream=None)
+    tuned.update(variant=18, stream=None)
     # shapes that a kernel cannot run, and numbers that name none
-    refused(pkg.lib().fp8gemm_grouped_tuned, tuned, [dict(variant=1), dict(variant=14), dict(variant=99), dict(variant=13, k=128), dict(variant=6, k=100), dict(variant=15, a=ODD), dict(variant=5, k=(1 << 23) + 16)])
+    refused(pkg.lib().fp8gemm_grouped_tuned, tuned, [dict(variant=1), dict(variant=5), dict(variant=99), dict(variant=13, k=128), dict(variant=14, k=272), dict(variant=18, k=100), dict(variant=15, a=ODD), dict(variant=13, k=(1 << 23) + 16)])
 
 
 def test_wgrad(pkg):
@@ -43,8 +43,8 @@ def test_wgrad(pkg):
     refused(pkg.lib().fp8gemm_grouped_wgrad, WGRAD, changes)
     tuned = dict(WGRAD)
     del tuned["stream"]
-    tuned.update(variant=6, stream=None)
-    refused(pkg.lib().fp8gemm_grouped_wgrad_tuned, tuned, [dict(variant=0), dict(variant=5), dict(variant=15)])
+    tuned.update(variant=18, stream=None)
+    refused(pkg.lib().fp8gemm_grouped_wgrad_tuned, tuned, [dict(variant=0), dict(variant=5), dict(variant=17)])
 
 
 def test_quantize(pkg):
