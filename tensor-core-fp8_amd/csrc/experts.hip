@@ -10,7 +10,7 @@
 
 #include "dispatch.h"
 #include "kernel_quantize.h"
-#include "kernel_w4.h"
+#include "w4_args.h"
 
 namespace fp8gemm_detail {
 
@@ -79,6 +79,14 @@ int plan_wgrad(int rows, int groups)
     return rows / groups < 512 ? 18 : 13;
 }
 
+}  // namespace fp8gemm_detail
+
+namespace fp8gemm_detail {
+extern template hipError_t launch_w4<true, kW4Int>(const W4Args &, hipStream_t);
+extern template hipError_t launch_w4<false, kW4Int>(const W4Args &, hipStream_t);
+extern template hipError_t launch_w4<true, kW4Fp4>(const W4Args &, hipStream_t);
+extern template hipError_t launch_w4<false, kW4Fp4>(const W4Args &, hipStream_t);
+extern template hipError_t launch_w4<false, kW4Fp4Scaled>(const W4Args &, hipStream_t);
 }  // namespace fp8gemm_detail
 
 using namespace fp8gemm_detail;
@@ -175,48 +183,6 @@ bool quantize_source_ok(int rows, int cols, const void *x, int x_type, long long
 }
 
 // ------------------------------------------------------------------ 4-bit weights
-template <bool F16, int MODE, int RUN, int MT>
-struct W4KernelTag {};
-
-constexpr int kW4MaxLds = 160 * 1024;
-
-template <bool F16, int MODE, int RUN, int MT>
-hipError_t launch_w4_kernel(W4Args p, hipStream_t s)
-{
-    const int most_rows = std::min(p.rows, 16 * MT);
-    const int col_tiles = (p.n + 15) / 16;
-    // Waves along K until the grid has two workgroups for every CU, as long as each keeps a few ring stages of K.
-    int wk = 1;
-    while (wk < kW4Waves && (long)((col_tiles + kW4Waves / wk - 1) / (kW4Waves / wk)) * p.groups < 512 && p.k >= 4 * wk * kW4StageK) wk *= 2;
-    p.wk = wk;
-    const int wc = kW4Waves / wk;
-    // k staged at a time: all of it, or as much as leaves room for a second workgroup on the CU
-    const int unit = kW4StageK * wk;
-    int chunk = (p.k + unit - 1) / unit * unit;
-    while (chunk > unit && kW4RingBytes + w4_stage_bytes(most_rows, chunk, wc, RUN, p.zeros != nullptr) > kW4MaxLds / 2) {
-        chunk = (chunk / 2 + unit - 1) / unit * unit;
-    }
-    p.chunk = chunk;
-    const int parts = wk > 1 ? (wk - 1) * wc * MT * 1024 : 0;
-    const int lds = kW4RingBytes + std::max(w4_stage_bytes(most_rows, chunk, wc, RUN, p.zeros != nullptr), parts);
-    if (lds > kW4MaxLds) return hipErrorInvalidValue;
-    auto kernel = gemv_w4_kernel<F16, MODE, RUN, MT>;
-    hipError_t e = allow_lds<W4KernelTag<F16, MODE, RUN, MT>>(kernel, kW4MaxLds);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((p.n + 16 * wc - 1) / (16 * wc)), (unsigned)p.groups), dim3(64 * kW4Waves), lds, s, p);
-    return hipGetLastError();
-}
-
-template <bool F16, int MODE, int RUN>
-hipError_t launch_w4_rows(const W4Args &p, hipStream_t s)
-{
-    // rows of x per pass over the weights; with experts, what an expert has on average
-    const int average = (p.rows + p.groups - 1) / p.groups;
-    if (p.rows <= 16 || average <= 8) return launch_w4_kernel<F16, MODE, RUN, 1>(p, s);
-    if (p.rows <= 32 || average <= 16) return launch_w4_kernel<F16, MODE, RUN, 2>(p, s);
-    return launch_w4_kernel<F16, MODE, RUN, 4>(p, s);
-}
-
 int gemv_w4(int groups, int m, int k, int n, const int *row_offsets, const void *x, int x_type, const float *x_scale, const void *w, int w_fmt, int run,
             const void *w_scales, int scale_type, const void *w_zeros, void *y, int y_type, void *stream)
 {
@@ -229,21 +195,17 @@ int gemv_w4(int groups, int m, int k, int n, const int *row_offsets, const void 
     if (!wide_ok(y_type) || !wide_aligned(y, y_type) || !aligned_to(x, 16) || !aligned_to(w, 16)) return (int)hipErrorInvalidValue;
     if (wide_ok(scale_type) && !wide_aligned(w_scales, scale_type)) return (int)hipErrorInvalidValue;
     const W4Args p = {row_offsets, groups, m, k, n, x, x_type, x_scale, static_cast<const uint8_t *>(w), w_scales, scale_type,
-                      static_cast<const uint8_t *>(w_zeros), run, y, y_type, 0, 1};
+                      static_cast<const uint8_t *>(w_zeros), run, y, y_type, k / run, 0, 1, 0, 0, 0, 1, 0};
     hipStream_t s = static_cast<hipStream_t>(stream);
     (void)hipGetLastError();
-    const bool f16 = x_type != FP8GEMM_T_BF16, long_runs = run % 128 == 0;
+    const bool f16 = x_type != FP8GEMM_T_BF16;
     hipError_t e;
-    if (w_fmt == FP8GEMM_W4_INT) {
-        if (f16)
-            e = long_runs ? launch_w4_rows<true, kW4Int, 128>(p, s) : launch_w4_rows<true, kW4Int, 32>(p, s);
-        else
-            e = long_runs ? launch_w4_rows<false, kW4Int, 128>(p, s) : launch_w4_rows<false, kW4Int, 32>(p, s);
-    } else if (f16) {
-        e = long_runs ? launch_w4_rows<true, kW4Fp4, 128>(p, s) : launch_w4_rows<true, kW4Fp4, 32>(p, s);
-    } else {
-        e = long_runs ? launch_w4_rows<false, kW4Fp4, 128>(p, s) : launch_w4_rows<false, kW4Fp4, 32>(p, s);
-    }
+    if (w_fmt == FP8GEMM_W4_INT)
+        e = f16 ? launch_w4<true, kW4Int>(p, s) : launch_w4<false, kW4Int>(p, s);
+    else if (f16)
+        e = launch_w4<true, kW4Fp4>(p, s);
+    else
+        e = scale_type == FP8GEMM_T_E8M0 ? launch_w4<false, kW4Fp4Scaled>(p, s) : launch_w4<false, kW4Fp4>(p, s);
     return (int)e;
 }
 

@@ -8,7 +8,8 @@
 // to the expansion, one instruction per weight:
 //   integers: a nibble q is masked into the mantissa of 16.0, which makes 16 + q; a second MFMA on the same x
 //     with -(16 + zero) in place of W takes the excess out (all exact: small integers in 16 bits, sums in fp32),
-//     so zero points cost no instruction per weight;
+//     so zero points cost no instruction per weight (taking it out as (16 + zero) times the sum of the run's x
+//     saves those MFMAs and loses more at the staging of x, from four rows on by a factor);
 //   e2m1: the conversion instruction, two weights at a time, which also applies power-of-two scales where
 //     x is bf16 (exact: bf16 has fp32's exponents).
 // Other scales multiply the fp32 sum of a run, so neither weights nor scales are rounded.
@@ -17,58 +18,29 @@
 // consecutive weights with one 16-byte LDS read.  Shorter runs: the four lanes of a row share 32 consecutive
 // weights, so that an MFMA stays inside one run.
 //
-// A workgroup of four waves is WC waves side by side (16 columns each) times WK waves along K, whose sums are
-// added in wave order through LDS at the end: few columns still fill the chip.  x and the scales of `chunk` k
-// at a time are staged in LDS for all four.
+// A workgroup of eight waves is WC waves side by side (16 columns each) times WK waves along K, whose sums are
+// added in wave order through LDS: few columns still fill the chip.  It goes through several blocks of columns;
+// x and the scales of all of them are staged in LDS once, then the waves' rings run without a break over all blocks.
 #ifndef FP8GEMM_KERNEL_W4_H
 #define FP8GEMM_KERNEL_W4_H
 
 #include "kernel_ptile.h"
 #include "kernel_skinny.h"
+#include "w4_args.h"
 
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
-constexpr int kW4Waves = 4;
+constexpr int kW4Waves = 8, kW4WavesShift = 3;         // of a workgroup
 constexpr int kW4RowBytes = 128;                       // of a row of W per ring stage: 256 weights
-constexpr int kW4Stages = 5;
 constexpr int kW4StageK = 2 * kW4RowBytes;
 constexpr int kW4StageBytes = 16 * kW4RowBytes;
 constexpr int kW4StageLoads = kW4StageBytes / 1024;
-constexpr int kW4RingBytes = kW4Waves * kW4Stages * kW4StageBytes;
+constexpr int kW4RingTwo = 2, kW4RingFour = 4;          // slots of a wave's ring: what fits
+__host__ __device__ constexpr int w4_ring_bytes(int slots) { return kW4Waves * slots * kW4StageBytes; }
 
-// how the weights become 16-bit numbers
-constexpr int kW4Int = 0;           // 16 + q, corrected by a second MFMA
-constexpr int kW4Fp4 = 1;           // e2m1, scales applied to sums
-constexpr int kW4Fp4Scaled = 2;     // e2m1, power-of-two scales applied by the conversion (bf16 only)
-
-struct W4Args {
-    const int *offsets;             // null: one group of all rows
-    int groups, rows;
-    int k, n;
-    const void *x;
-    int x_type;                     // FP8GEMM_T_*
-    const float *x_scale;
-    const uint8_t *w;
-    const void *w_scale;
-    int scale_type;
-    const uint8_t *zeros;
-    int run;
-    void *y;
-    int y_type;
-    int chunk;                      // k staged at a time: a multiple of kW4StageK * WK
-    int wk;
-};
-
-// one scale as a float
-__device__ __forceinline__ float w4_scale(const void *p, size_t i, int type)
-{
-    if (type == FP8GEMM_T_E8M0) {
-        const uint32_t b = static_cast<const uint8_t *>(p)[i];
-        return __builtin_bit_cast(float, b == 0 ? 0x00400000u : (b == 255 ? 0x7FC00000u : b << 23));
-    }
-    return load_in(p, i, type);
-}
+// how the scales lie in LDS: as they are stored, bytes as bf16 (the same powers of two) where a sum is multiplied
+constexpr int kW4ScaleF32 = 0, kW4ScaleBf16 = 1, kW4ScaleF16 = 2, kW4ScaleByte = 3;
 
 template <bool F16, int MODE>
 __device__ __forceinline__ v4i w4_expand(uint32_t w, float scale)
@@ -76,17 +48,15 @@ __device__ __forceinline__ v4i w4_expand(uint32_t w, float scale)
     v4i r;
     if constexpr (MODE == kW4Int) {
         // the nibbles of each 16-bit half, lowest first, into the mantissa's top four bits of 16.0
-        if constexpr (F16) {
-            r[0] = (int)(((w << 6) & 0x03C003C0u) | 0x4C004C00u);
-            r[1] = (int)(((w << 2) & 0x03C003C0u) | 0x4C004C00u);
-            r[2] = (int)(((w >> 2) & 0x03C003C0u) | 0x4C004C00u);
-            r[3] = (int)(((w >> 6) & 0x03C003C0u) | 0x4C004C00u);
-        } else {
-            r[0] = (int)(((w << 3) & 0x00780078u) | 0x41804180u);
-            r[1] = (int)(((w >> 1) & 0x00780078u) | 0x41804180u);
-            r[2] = (int)(((w >> 5) & 0x00780078u) | 0x41804180u);
-            r[3] = (int)(((w >> 9) & 0x00780078u) | 0x41804180u);
-        }
+        // (mask and exponent kept in registers, one of each kind: the and-or takes no literals)
+        uint32_t mask = F16 ? 0x03C003C0u : 0x00780078u, sixteen = F16 ? 0x4C004C00u : 0x41804180u;
+        asm("" : "+s"(mask));
+        asm("" : "+v"(sixteen));
+        constexpr int UP = F16 ? 6 : 3;                   // from bit 0 to the mantissa's top
+        r[0] = (int)(((w << UP) & mask) | sixteen);
+        r[1] = (int)(((UP >= 4 ? w << (UP >= 4 ? UP - 4 : 0) : w >> (UP >= 4 ? 0 : 4 - UP)) & mask) | sixteen);
+        r[2] = (int)(((w >> (8 - UP)) & mask) | sixteen);
+        r[3] = (int)(((w >> (12 - UP)) & mask) | sixteen);
     } else if constexpr (F16) {
         r[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0));
         r[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1));
@@ -135,26 +105,168 @@ __device__ __forceinline__ v4i w4_load_x(const void *x, size_t index, int type)
     return r;
 }
 
-// LDS behind the ring for `rows` rows of x, `chunk` k and wc waves side by side; scales once per RUN k
-constexpr int w4_stage_bytes(int rows, int chunk, int wc, int run_k, bool zeros)
+// Staged x and scales.  x: a row behind the other, 16 bytes apart in the banks; scales: a column behind the other, an entry per run
+// of RUN k -- the scale and, for integers, -(16 + zero) beside it in 16 bits -- odd counts of 16 bytes apart.  A lane's reads
+// then differ by constants that the instructions carry, and 16 lanes read 16 rows or columns without a conflict.
+__host__ __device__ constexpr int w4_entry_bytes(int mode, int kind)
 {
-    return rows * chunk * 2 + (chunk / run_k) * 16 * wc * 4 * (zeros ? 2 : 1);
+    return kind == kW4ScaleByte ? 1 : (kind == kW4ScaleF32 ? 4 : 2) * (mode == kW4Int ? 2 : 1);
+}
+__host__ __device__ constexpr int w4_x_pitch(int chunk) { return chunk * 2 + 16; }
+__host__ __device__ constexpr int w4_scale_pitch(int runs, int entry) { return ((runs * entry + 15) / 16 | 1) * 16; }
+// two sets of the partial sums of the waves along K: rows x 16 floats a wave
+__host__ __device__ constexpr int w4_part_bytes(int wk, int rows) { return wk > 1 ? 2 * (wk - 1) * (kW4Waves / wk) * rows * 64 : 0; }
+
+// -(16 + z) in 16 bits, twice: z in the top of the mantissa of -16
+template <bool F16>
+__device__ __forceinline__ uint32_t w4_excess(uint32_t z)
+{
+    return F16 ? 0xCC00CC00u | (z << 6) | (z << 22) : 0xC180C180u | (z << 3) | (z << 19);
+}
+// the staged entry of a stored scale (its bits) and zero point (fp32 scales: the scale alone)
+template <bool F16, int MODE, int KIND, int ES>
+__device__ __forceinline__ uint32_t w4_pack_entry(uint32_t bits, uint32_t z)
+{
+    // (a byte b stands for 2^(b - 127); as bf16 that is b << 7, 0 the subnormal 0x0040 and 255 a NaN.  The conversion takes
+    // the byte as it is.)
+    if (ES == 1 && KIND == kW4ScaleBf16) bits = bits == 0 ? 0x0040u : (bits == 255 ? 0x7FC0u : bits << 7);
+    if (MODE == kW4Int && KIND != kW4ScaleF32) bits |= w4_excess<F16>(z) & 0xFFFF0000u;
+    return bits;
+}
+
+// Stages the scales (and zero points) of `block_cols` columns for k from first_k on, `runs` staged runs each, by `threads` threads.
+// ES: bytes of a stored scale; VEC: a stored run is a staged run and 16 bytes of scales can be read at once.  Columns from
+// `cols` on and what lies behind the last k are staged as zeros (x is zero there, or nothing is stored).
+template <bool F16, int MODE, int RUN, int KIND, int ES, bool VEC>
+__device__ __forceinline__ void w4_stage_scales(const W4Args &p, size_t at0, int first_k, int runs, int cols, int block_cols, LDS_AS uint8_t *out, int tid, int threads)
+{
+    constexpr int EB = w4_entry_bytes(MODE, KIND);
+    constexpr int E = VEC ? 16 / ES : 1;                  // scales a thread takes at once
+    constexpr int BATCH = 2;                              // ... and how many such loads it has in flight
+    const int pitch = w4_scale_pitch(runs, EB);
+    const int units = (runs + E - 1) / E;                 // of a column, dealt to a power of two of threads
+    const int shift = units > 32 ? 6 : (units > 1 ? 32 - __builtin_clz(units - 1) : 0);
+    const int sub = tid & ((1 << shift) - 1), cols_at_once = threads >> shift;
+    for (int unit = sub; unit < units; unit += 1 << shift)
+        for (int col0 = tid >> shift; col0 < block_cols; col0 += BATCH * cols_at_once) {
+            const int at_k = first_k + unit * E * RUN;
+            const size_t at_row = VEC ? (size_t)(first_k / RUN + unit * E) : (size_t)(at_k / p.run);
+            v4i raw[BATCH], z[BATCH];                     // (not VEC: one scale, one zero point, in the lowest bits)
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                const int col = col0 + b * cols_at_once;
+                raw[b] = z[b] = v4i{0, 0, 0, 0};
+                if (col < cols && at_k < p.k) {           // (VEC: E divides what a row holds, all of them or none)
+                    const size_t at = at0 + (size_t)col * p.per_row + at_row;
+                    const uint8_t *from = static_cast<const uint8_t *>(p.w_scale) + at * ES;
+                    if constexpr (VEC)
+                        raw[b] = *reinterpret_cast<const v4i *>(from);
+                    else
+                        raw[b][0] = ES == 4 ? *reinterpret_cast<const int *>(from) : (ES == 2 ? *reinterpret_cast<const unsigned short *>(from) : *from);
+                    if (MODE == kW4Int) {
+                        if (!p.zeros) {
+                            z[b] = v4i{0x08080808, 0x08080808, 0x08080808, 0x08080808};
+                        } else if constexpr (E == 1) {
+                            z[b][0] = p.zeros[at];
+                        } else if constexpr (E == 4) {
+                            z[b][0] = *reinterpret_cast<const int *>(p.zeros + at);
+                        } else if constexpr (E == 8) {
+                            const v2u t = *reinterpret_cast<const v2u *>(p.zeros + at);
+                            z[b][0] = (int)t[0];
+                            z[b][1] = (int)t[1];
+                        } else {
+                            z[b] = *reinterpret_cast<const v4i *>(p.zeros + at);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                const int col = col0 + b * cols_at_once;
+                if (col >= block_cols) continue;
+                LDS_AS uint8_t *to = out + col * pitch + unit * E * EB;
+                if constexpr (KIND == kW4ScaleByte) {     // the bytes as they are
+                    if constexpr (VEC)
+                        *reinterpret_cast<LDS_AS v4i *>(to) = raw[b];
+                    else
+                        *to = (uint8_t)raw[b][0];
+                    continue;
+                }
+                // (VEC: a column's pitch has room for whole units)
+                v4i word = {0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const uint32_t part = (uint32_t)raw[b][e * ES / 4] >> (8 * (e * ES % 4));
+                    const uint32_t bits = ES == 4 ? part : part & (ES == 2 ? 0xFFFFu : 0xFFu);
+                    const uint32_t zero = ((uint32_t)z[b][e / 4] >> (8 * (e & 3))) & 15u;
+                    const uint32_t entry = w4_pack_entry<F16, MODE, KIND, ES>(bits, zero);
+                    if constexpr (EB == 8) {
+                        word[2 * (e & 1)] = (int)entry;
+                        word[2 * (e & 1) + 1] = (int)w4_excess<F16>(zero);
+                        if (!VEC) *reinterpret_cast<LDS_AS v2u *>(to) = v2u{(uint32_t)word[0], (uint32_t)word[1]};
+                        if (VEC && (e & 1)) *reinterpret_cast<LDS_AS v4i *>(to + (e - 1) * EB) = word;
+                    } else if constexpr (EB == 4) {
+                        word[e & 3] = (int)entry;
+                        if (!VEC) *reinterpret_cast<LDS_AS uint32_t *>(to) = entry;
+                        if (VEC && (e & 3) == 3) *reinterpret_cast<LDS_AS v4i *>(to + (e - 3) * EB) = word;
+                    } else {
+                        if (!VEC) *reinterpret_cast<LDS_AS unsigned short *>(to) = (unsigned short)entry;
+                        if (VEC) {
+                            word[(e & 7) / 2] = (e & 1) ? (int)((uint32_t)word[(e & 7) / 2] | (entry << 16)) : (int)entry;
+                            if ((e & 7) == 7) *reinterpret_cast<LDS_AS v4i *>(to + (e - 7) * EB) = word;
+                        }
+                    }
+                }
+            }
+        }
+}
+
+// an entry of the staged scales: the scale, and for integers the 16-bit -(16 + zero) twice
+template <int MODE, int KIND>
+__device__ __forceinline__ void w4_entry(const LDS_AS uint8_t *at, float &scale, uint32_t &excess)
+{
+    uint32_t bits;
+    if constexpr (MODE == kW4Int && KIND == kW4ScaleF32) {
+        const v2u e = *reinterpret_cast<const LDS_AS v2u *>(at);
+        bits = e[0];
+        excess = e[1];
+    } else if constexpr (MODE == kW4Int) {
+        bits = *reinterpret_cast<const LDS_AS uint32_t *>(at);
+        excess = __builtin_amdgcn_perm(bits, bits, 0x03020302u);
+    } else if constexpr (KIND == kW4ScaleF32) {
+        bits = *reinterpret_cast<const LDS_AS uint32_t *>(at);
+    } else if constexpr (KIND == kW4ScaleByte) {
+        bits = *at;
+    } else {
+        bits = *reinterpret_cast<const LDS_AS unsigned short *>(at);
+    }
+    if constexpr (KIND == kW4ScaleF32)
+        scale = __builtin_bit_cast(float, bits);
+    else if constexpr (KIND == kW4ScaleBf16)
+        scale = __builtin_bit_cast(float, bits << 16);
+    else if constexpr (KIND == kW4ScaleF16)
+        scale = (float)__builtin_bit_cast(_Float16, (unsigned short)bits);
+    else
+        scale = __builtin_bit_cast(float, bits << 23);
 }
 
 // F16: x and the expanded weights are f16 (else bf16).  RUN: 128 or 32, the k between two scales of the staged table.
 // MT: blocks of 16 rows of x held at once.
-template <bool F16, int MODE, int RUN, int MT>
+// KIND: how the scales are staged.
+template <bool F16, int MODE, int RUN, int MT, int KIND>
 __global__ __launch_bounds__(64 * kW4Waves) void gemv_w4_kernel(W4Args p)
 {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const uint32_t lds_base = (uint32_t)(uintptr_t)(LDS_AS uint8_t *)lds;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int wc_count = kW4Waves / p.wk;
-    const int wc = wave % wc_count, wk = wave / wc_count;
+    const int wk_count = 1 << p.wk_shift, wc_count = kW4Waves >> p.wk_shift;
+    const int wc = wave & (wc_count - 1), wk = wave >> (kW4WavesShift - p.wk_shift);
     const int g = blockIdx.y;
     const int block_cols = 16 * wc_count;
-    const int block_n0 = blockIdx.x * block_cols;
+    // this workgroup's blocks of columns, one behind the other
+    const int block_n0 = blockIdx.x * block_cols * p.blocks;
+    const int blocks = p.n - block_n0 < p.blocks * block_cols ? (p.n - block_n0 + block_cols - 1) >> (4 + kW4WavesShift - p.wk_shift) : p.blocks;
     const int n0 = block_n0 + 16 * wc;
     int first = 0, end = p.rows;
     if (p.offsets) {
@@ -180,7 +292,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemv_w4_kernel(W4Args p)
 
     // ---- ring of this wave: 16 rows of W, kW4RowBytes of each a stage, 16-byte pieces swizzled by row
     const size_t row_bytes = (size_t)p.k / 2;
-    const int rows_w = p.n - n0 < 16 ? (p.n - n0 < 0 ? 0 : p.n - n0) : 16;
+    const int rows_w = p.n - n0 < 0 ? 0 : p.n - n0;
     // (rows past the last column of y, and bytes past the end of the last row, fall outside the extent and read as zeros;
     // bytes past the end of other rows are the next row's: x is zero there)
     const v4i rs = make_buffer_resource(p.w + ((size_t)g * p.n + (rows_w ? n0 : 0)) * row_bytes, (unsigned long long)rows_w * row_bytes);
@@ -190,156 +302,270 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemv_w4_kernel(W4Args p)
         const int row = j * 8 + (lane >> 3);
         ld_off[j] = (uint32_t)row * (uint32_t)row_bytes + (uint32_t)(((lane & 7) ^ (skinny_swizzle<kW4RowBytes>(row) & 7)) * 16);
     }
-    const uint32_t ring = lds_base + (uint32_t)(wave * kW4Stages * kW4StageBytes);
-    const uint8_t *ring_ptr = lds + wave * kW4Stages * kW4StageBytes;
+    const uint32_t ring = lds_base + (uint32_t)(wave * p.ring * kW4StageBytes);
     const int sw = skinny_swizzle<kW4RowBytes>(fi) & 7;
-    auto issue = [&](int k0, int stage) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < kW4StageLoads; ++j)
-            buffer_load_lds_b128_stream(rs, ring + (uint32_t)(stage * kW4StageBytes + j * 1024), ld_off[j] + (uint32_t)(k0 / 2), 0u);
-    };
+    const LDS_AS uint8_t *ring_ptr = (const LDS_AS uint8_t *)lds + wave * p.ring * kW4StageBytes + fi * kW4RowBytes;
+    LDS_AS float *parts = (LDS_AS float *)((LDS_AS uint8_t *)lds + w4_ring_bytes(p.ring));
+    LDS_AS uint8_t *xs = (LDS_AS uint8_t *)lds + w4_ring_bytes(p.ring) + w4_part_bytes(wk_count, p.part_rows);
+    constexpr bool PER_LANE = RUN == 128 || MODE == kW4Fp4Scaled;     // a lane has 32 consecutive weights
+    constexpr int EB = w4_entry_bytes(MODE, KIND), RUNS128 = 128 / RUN;
+    const int unit = kW4StageK << p.wk_shift;
+    const int whole = (p.k + unit - 1) & ~(unit - 1);
+    int flushed = 0;                                      // tiles added up so far: which of the two sets of partial sums is next
 
-    uint8_t *xs = lds + kW4RingBytes;
-    const int slice = p.chunk / p.wk;                     // k of a chunk that this wave multiplies
     for (int m0 = first; m0 < end; m0 += 16 * MT) {
         const int rows = end - m0 < 16 * MT ? end - m0 : 16 * MT;
+        // Staged at a time: all of K of x, and the scales of as many blocks of columns as fit beside it; where not even one
+        // does, a block at a time with K in equal pieces, whole ring stages for every wave along K (the host leaves room
+        // for one), whole multiples of 2048 if they are longer.
+        // (as planned, unless an expert has more rows than the plan took it to have)
+        int chunk = whole, pass = p.pass;
+        if (rows > p.plan_rows || pass == 0) {
+            pass = (p.stage_bytes - rows * w4_x_pitch(whole)) / (block_cols * w4_scale_pitch(whole / RUN, EB));
+            if (pass < 1) {
+                // (what a run takes, and the padding of rows and columns)
+                const int per_run = rows * RUN * 2 + block_cols * EB;
+                const int most_k = (p.stage_bytes - rows * 16 - block_cols * 31) / per_run * RUN;
+                const int step = most_k >= 2048 ? 2048 : unit;
+                const int most = most_k / step * step, pieces = (p.k + most - 1) / most;
+                chunk = ((p.k + pieces - 1) / pieces + step - 1) / step * step;
+                pass = 1;
+            }
+        }
+        chunk = __builtin_amdgcn_readfirstlane(chunk);
+        pass = __builtin_amdgcn_readfirstlane(pass);
+        const int runs = chunk / RUN, x_pitch = w4_x_pitch(chunk), s_pitch = w4_scale_pitch(runs, EB);
+        int x_row[MT];                                    // this lane's place in the staged x (past the last row: that one again)
+        float x_scale[MT][4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            x_row[i] = (i * 16 + fi < rows ? i * 16 + fi : rows - 1) * x_pitch + (PER_LANE ? 4 * fq : fq) * 16;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = i * 16 + 4 * fq + r;
+                x_scale[i][r] = p.x_scale && row < rows ? p.x_scale[m0 + row] : 1.0f;
+            }
+        }
         v4f total[MT];
+        for (int b0 = 0; b0 < blocks; b0 += pass) {
+            const int nb = blocks - b0 < pass ? blocks - b0 : pass;
+            for (int c0 = 0; c0 < p.k; c0 += chunk) {
+                // Ring stages of K are dealt to the waves along K in turn, so that they read neighbouring lines; every workgroup
+                // starts at its own one (workgroups in step would ask the same HBM channels at the same time).
+                const int ks = ((p.k - c0 < chunk ? p.k - c0 : chunk) + kW4StageK - 1) / kW4StageK;
+                const int T = ks > wk ? (ks - wk + wk_count - 1) >> p.wk_shift : 0;
+                const int rot = T > 1 ? (int)(((((unsigned)(blockIdx.x + b0) * 2654435761u) >> 16) * (unsigned)T) >> 16) : 0;      // < T
+                int next_b = 0, next_t = 0, left = nb * T;   // the next stage to load, and how many are left
+                auto issue = [&](int stage) __attribute__((always_inline)) {
+                    int t = next_t + rot;
+                    t = t >= T ? t - T : t;
+                    const uint32_t at = (uint32_t)(b0 + next_b) * (uint32_t)block_cols * (uint32_t)row_bytes + (uint32_t)((c0 + ((t << p.wk_shift) + wk) * kW4StageK) / 2);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) total[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int c0 = 0; c0 < p.k; c0 += p.chunk) {
-            const int kw0 = c0 + wk * slice;
-            const int left = p.k - kw0 < slice ? p.k - kw0 : slice;
-            const int T = left > 0 ? (left + kW4StageK - 1) / kW4StageK : 0;
-            __syncthreads();                              // (the staged x and scales of the chunk before are done with)
-#pragma unroll
-            for (int t = 0; t < kW4Stages - 1; ++t)
-                if (t < T) issue(kw0 + t * kW4StageK, t);
-            // ---- x and the scales of the chunk
-            const int units = p.chunk / 8;                // eight numbers of a row; laid out [unit][row]
-            for (int u = threadIdx.x; u < units * rows; u += 64 * kW4Waves) {
-                const int unit = u / rows, row = u - unit * rows;
-                const int kk = c0 + unit * 8;
-                v4i v = {0, 0, 0, 0};
-                if (kk < p.k) v = w4_load_x<F16>(p.x, (size_t)(m0 + row) * p.k + kk, p.x_type);
-                if (MODE == kW4Int) {
-                    // in the order of the expanded nibbles: 0 4, 1 5, 2 6, 3 7
-                    const v4i o = v;
-                    v[0] = (int)(((uint32_t)o[0] & 0xFFFFu) | ((uint32_t)o[2] << 16));
-                    v[1] = (int)(((uint32_t)o[0] >> 16) | ((uint32_t)o[2] & 0xFFFF0000u));
-                    v[2] = (int)(((uint32_t)o[1] & 0xFFFFu) | ((uint32_t)o[3] << 16));
-                    v[3] = (int)(((uint32_t)o[1] >> 16) | ((uint32_t)o[3] & 0xFFFF0000u));
-                }
-                *reinterpret_cast<v4i *>(xs + (size_t)u * 16) = v;
-            }
-            float *ss = reinterpret_cast<float *>(xs + (size_t)units * rows * 16);
-            uint32_t *zs = reinterpret_cast<uint32_t *>(ss + (p.chunk / RUN) * block_cols);
-            const int runs = p.chunk / RUN, per_row = p.k / p.run;
-            for (int u = threadIdx.x; u < runs * block_cols; u += 64 * kW4Waves) {
-                const int col = u / runs, r = u - col * runs;
-                const int kk = c0 + r * RUN;
-                float s = MODE == kW4Fp4Scaled ? 1.0f : 0.0f;
-                uint32_t z = 0;
-                if (kk < p.k && block_n0 + col < p.n) {
-                    const size_t at = ((size_t)g * p.n + block_n0 + col) * per_row + kk / p.run;
-                    s = w4_scale(p.w_scale, at, p.scale_type);
-                    if (MODE == kW4Int && p.zeros) z = p.zeros[at] & 15u;
-                }
-                ss[r * block_cols + col] = s;
-                if (MODE == kW4Int && p.zeros) {
-                    const float c = -(16.0f + (float)z);
-                    const uint32_t h = out_bits16(c, F16 ? FP8GEMM_DEV_OUT_F16 : FP8GEMM_DEV_OUT_BF16);
-                    zs[r * block_cols + col] = h | (h << 16);
-                }
-            }
-            __syncthreads();
-            // ---- this wave's slice of the chunk
-            for (int t = 0; t < T; ++t) {
-                if (t + kW4Stages - 1 < T) {
-                    issue(kw0 + (t + kW4Stages - 1) * kW4StageK, (t + kW4Stages - 1) % kW4Stages);
-                    wait_vmcnt<kW4StageLoads *(kW4Stages - 1)>();
-                } else {
-                    wait_vmcnt<0>();
-                }
-                asm volatile("" ::: "memory");            // (the ring is written behind the compiler's back)
-                const uint8_t *st = ring_ptr + (t % kW4Stages) * kW4StageBytes + fi * kW4RowBytes;
-#pragma unroll
-                for (int h = 0; h < kW4StageK / 128; ++h) {           // 128 k: 64 bytes of a row, four 16-byte pieces
-                    const int k128 = (kw0 - c0 + t * kW4StageK) / 128 + h;
-                    uint32_t w[4];
-                    if constexpr (RUN == 128 || MODE == kW4Fp4Scaled) {
-                        const v4i v = *reinterpret_cast<const v4i *>(st + ((h * 4 + fq) ^ sw) * 16);
-#pragma unroll
-                        for (int d = 0; d < 4; ++d) w[d] = (uint32_t)v[d];
-                    } else {
-#pragma unroll
-                        for (int d = 0; d < 4; ++d) w[d] = *reinterpret_cast<const uint32_t *>(st + ((h * 4 + d) ^ sw) * 16 + fq * 4);
+                    for (int j = 0; j < kW4StageLoads; ++j)
+                        buffer_load_lds_b128_stream(rs, ring + (uint32_t)(stage * kW4StageBytes + j * 1024), ld_off[j] + at, 0u);
+                    --left;
+                    if (++next_t == T) {
+                        next_t = 0;
+                        ++next_b;
                     }
-                    constexpr bool PER_LANE = RUN == 128 || MODE == kW4Fp4Scaled;     // a lane has 32 consecutive weights
-                    v4f sum[MT];
-                    float lane_scale = 1.0f;
-                    if constexpr (MODE == kW4Fp4Scaled) lane_scale = ss[(RUN == 128 ? k128 : k128 * 4 + fq) * block_cols + 16 * wc + fi];
+                };
+                __syncthreads();                          // (what was staged before is done with)
 #pragma unroll
-                    for (int d = 0; d < 4; ++d) {
-                        const v4i b = w4_expand<F16, MODE>(w[d], lane_scale);
-                        const int unit = k128 * 16 + (PER_LANE ? 4 * fq + d : 4 * d + fq);
-                        const bool open = RUN == 32 || d == 0;         // a new run of the staged scales begins
-                        v4i zc;
-                        if constexpr (MODE == kW4Int) {
-                            int one = F16 ? (int)0xCE00CE00u : (int)0xC1C0C1C0u;       // -24
-                            if (p.zeros) one = (int)zs[(RUN == 128 ? k128 : k128 * 4 + d) * block_cols + 16 * wc + fi];
-                            zc = v4i{one, one, one, one};
-                        }
+                for (int t = 0; t < kW4RingFour; ++t)
+                    if (t < p.ring && left > 0) issue(t);
+                // x by the lower half of the waves and the scales by the upper half at the same time (all of them where x stays)
+                const bool with_x = b0 == 0 || chunk < whole;
+                const int half = 32 * kW4Waves;
+                if (with_x && threadIdx.x < half) {
+                    const int units = chunk / 8;          // eight numbers of a row
+                    constexpr int XB = 4;                 // loads a thread has in flight
+                    // (pieces of eight numbers, row after row; a thread's place moves on by `half` pieces)
+                    int row = 0, u = threadIdx.x;
+                    while (u >= units) {
+                        u -= units;
+                        ++row;
+                    }
+                    while (row < rows) {
+                        v4i v[XB];
+                        int at[XB];
 #pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            int row = i * 16 + fi;
-                            row = row < rows ? row : rows - 1;
-                            const v4i a = *reinterpret_cast<const v4i *>(xs + ((size_t)unit * rows + row) * 16);
-                            if constexpr (MODE == kW4Fp4Scaled) {
-                                total[i] = w4_mfma<F16>(a, b, total[i]);
-                            } else {
-                                sum[i] = w4_mfma<F16>(a, b, open ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : sum[i]);
-                                if constexpr (MODE == kW4Int) sum[i] = w4_mfma<F16>(a, zc, sum[i]);
+                        for (int b = 0; b < XB; ++b) {
+                            v[b] = v4i{0, 0, 0, 0};
+                            at[b] = row < rows ? row * x_pitch + u * 16 : -1;
+                            if (row < rows && c0 + u * 8 < p.k) v[b] = w4_load_x<F16>(p.x, (size_t)(m0 + row) * p.k + c0 + u * 8, p.x_type);
+                            u += half;
+                            while (u >= units) {
+                                u -= units;
+                                ++row;
                             }
                         }
-                        if (MODE != kW4Fp4Scaled && (RUN == 32 || d == 3)) {
-                            const float s = ss[(RUN == 128 ? k128 : k128 * 4 + d) * block_cols + 16 * wc + fi];
+#pragma unroll
+                        for (int b = 0; b < XB; ++b) {
+                            if (MODE == kW4Int) {
+                                // in the order of the expanded nibbles: 0 4, 1 5, 2 6, 3 7
+                                const v4i o = v[b];
+                                v[b][0] = (int)__builtin_amdgcn_perm((uint32_t)o[2], (uint32_t)o[0], 0x05040100u);
+                                v[b][1] = (int)__builtin_amdgcn_perm((uint32_t)o[2], (uint32_t)o[0], 0x07060302u);
+                                v[b][2] = (int)__builtin_amdgcn_perm((uint32_t)o[3], (uint32_t)o[1], 0x05040100u);
+                                v[b][3] = (int)__builtin_amdgcn_perm((uint32_t)o[3], (uint32_t)o[1], 0x07060302u);
+                            }
+                            if (at[b] >= 0) *reinterpret_cast<LDS_AS v4i *>(xs + at[b]) = v[b];
+                        }
+                    }
+                }
+                LDS_AS uint8_t *ss = xs + rows * x_pitch;
+                if (!with_x || threadIdx.x >= half) {
+                    const int col0 = block_n0 + b0 * block_cols, staged = nb * block_cols;
+                    const int cols = p.n - col0 < staged ? p.n - col0 : staged;
+                    const size_t at0 = ((size_t)g * p.n + col0) * p.per_row;
+                    const int es = p.scale_type == FP8GEMM_T_E8M0 ? 1 : (p.scale_type == FP8GEMM_T_F32 ? 4 : 2), last = 16 / es - 1;
+                    const bool vec = p.run == RUN && ((p.per_row | runs | (c0 / RUN)) & last) == 0 &&
+                                     reinterpret_cast<uintptr_t>(p.w_scale) % 16 == 0 && (!p.zeros || reinterpret_cast<uintptr_t>(p.zeros) % 16 == 0);
+                    const int tid = with_x ? threadIdx.x - half : threadIdx.x, threads = with_x ? half : 2 * half;
+#define W4_STAGE(ES) \
+    (vec ? w4_stage_scales<F16, MODE, RUN, KIND, ES, true>(p, at0, c0, runs, cols, staged, ss, tid, threads) \
+         : w4_stage_scales<F16, MODE, RUN, KIND, ES, false>(p, at0, c0, runs, cols, staged, ss, tid, threads))
+                    if constexpr (KIND == kW4ScaleF32) {
+                        W4_STAGE(4);
+                    } else if constexpr (KIND == kW4ScaleByte) {
+                        W4_STAGE(1);
+                    } else {
+                        if (KIND == kW4ScaleBf16 && es == 1)
+                            W4_STAGE(1);
+                        else
+                            W4_STAGE(2);
+                    }
+#undef W4_STAGE
+                }
+                // (every load has landed: said here, so that the compiler does not wait for all of them inside the loop)
+                wait_vmcnt<0>();
+                __syncthreads();
+                // The weights of a stage are read from the ring into registers while those of the stage before are multiplied:
+                // the slot is free for another as soon as they are there.
+                uint32_t now[kW4StageK / 32], next[kW4StageK / 32];
+                auto read_stage = [&](int stage, uint32_t *w) __attribute__((always_inline)) {
+                    asm volatile("" ::: "memory");        // (the ring is written behind the compiler's back)
+                    const LDS_AS uint8_t *st = ring_ptr + stage * kW4StageBytes;
+#pragma unroll
+                    for (int h = 0; h < kW4StageK / 128; ++h) {       // 128 k: 64 bytes of a row, four 16-byte pieces
+                        if constexpr (PER_LANE) {
+                            const v4i v = *reinterpret_cast<const LDS_AS v4i *>(st + ((h * 4 + fq) ^ sw) * 16);
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) w[4 * h + d] = (uint32_t)v[d];
+                        } else {
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) w[4 * h + d] = *reinterpret_cast<const LDS_AS uint32_t *>(st + ((h * 4 + d) ^ sw) * 16 + fq * 4);
+                        }
+                    }
+                };
+                int stage = 0, todo = nb * T;
+                // (every load has landed, see above)
+                if (todo > 0) read_stage(0, now);
+                wait_lgkmcnt0();
+                for (int b = 0; b < nb; ++b) {
+                    if (c0 == 0)
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) total[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                    const LDS_AS uint8_t *s_block = ss + (b * block_cols + 16 * wc + fi) * s_pitch + (MODE == kW4Fp4Scaled && RUN == 32 ? fq : 0) * EB;
+                    for (int t0 = 0; t0 < T; ++t0) {
+                        if (left > 0) {
+                            issue(stage);
+                            if (p.ring == kW4RingTwo)
+                                wait_vmcnt<(kW4RingTwo - 1) * kW4StageLoads>();
+                            else
+                                wait_vmcnt<(kW4RingFour - 1) * kW4StageLoads>();
+                        } else {
+                            wait_vmcnt<0>();
+                        }
+                        stage = stage == p.ring - 1 ? 0 : stage + 1;
+                        if (--todo > 0) read_stage(stage, next);
+                        int t = t0 + rot;
+                        t = t >= T ? t - T : t;
+                        const int k_at = ((t << p.wk_shift) + wk) * kW4StageK;
+                        const LDS_AS uint8_t *x_at = xs + k_at * 2, *s_at = s_block + k_at / RUN * EB;
+#pragma unroll
+                        for (int h = 0; h < kW4StageK / 128; ++h) {
+                            const uint32_t *w = now + 4 * h;
+                            v4f sum[MT], excess[MT];
+                            float lane_scale = 1.0f, s = 0.0f;
+                            uint32_t pair = 0;
+                            v4i minus;
+                            if constexpr (MODE == kW4Fp4Scaled) w4_entry<MODE, KIND>(s_at + h * RUNS128 * EB, lane_scale, pair);
+#pragma unroll
+                            for (int d = 0; d < 4; ++d) {
+                                const v4i wide = w4_expand<F16, MODE>(w[d], lane_scale);
+                                const bool open = RUN == 32 || d == 0;         // a new run of the staged scales begins
+                                if constexpr (MODE != kW4Fp4Scaled)
+                                    if (open) {
+                                        w4_entry<MODE, KIND>(s_at + (h * RUNS128 + (RUN == 32 ? d : 0)) * EB, s, pair);
+                                        minus = v4i{(int)pair, (int)pair, (int)pair, (int)pair};
+                                    }
+#pragma unroll
+                                for (int i = 0; i < MT; ++i) {
+                                    const v4i a = *reinterpret_cast<const LDS_AS v4i *>(x_at + x_row[i] + h * 256 + (PER_LANE ? d : 4 * d) * 16);
+                                    if constexpr (MODE == kW4Fp4Scaled) {
+                                        total[i] = w4_mfma<F16>(a, wide, total[i]);
+                                    } else {
+                                        // (the excess in a chain of its own: the two do not wait for each other)
+                                        sum[i] = w4_mfma<F16>(a, wide, open ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : sum[i]);
+                                        if constexpr (MODE == kW4Int) excess[i] = w4_mfma<F16>(a, minus, open ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : excess[i]);
+                                    }
+                                }
+                                if (MODE != kW4Fp4Scaled && (RUN == 32 || d == 3)) {
+#pragma unroll
+                                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                                        for (int r = 0; r < 4; ++r) total[i][r] += s * (MODE == kW4Int ? sum[i][r] + excess[i][r] : sum[i][r]);
+                                }
+                            }
+                        }
+                        // all reads of the next stage have returned before its slot is refilled
+                        wait_lgkmcnt0();
+                        asm volatile("" ::: "memory");
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int d = 0; d < kW4StageK / 32; ++d) now[d] = next[d];
+                    }
+                    if (c0 + chunk < p.k) continue;
+                    // ---- the waves along K, added in wave order (two sets of partial sums in turn: one barrier a tile);
+                    // register r of lane (fi, fq) holds y[16 i + 4 fq + r][column fi]
+                    if (wk_count > 1) {
+                        LDS_AS float *set = parts + (flushed & 1) * ((wk_count - 1) * wc_count * p.part_rows * 16);
+                        ++flushed;
+                        if (wk > 0)
 #pragma unroll
                             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                                for (int r = 0; r < 4; ++r) total[i][r] += s * sum[i][r];
-                        }
+                                for (int r = 0; r < 4; ++r) {
+                                    const int row = i * 16 + 4 * fq + r;
+                                    if (row < rows) set[(((wk - 1) * wc_count + wc) * p.part_rows + row) * 16 + fi] = total[i][r];
+                                }
+                        wait_lgkmcnt0();
+                        asm volatile("" ::: "memory");
+                        __builtin_amdgcn_s_barrier();     // (the loads in flight go on)
+                        asm volatile("" ::: "memory");
+                        if (wk == 0)
+                            for (int o = 1; o < wk_count; ++o)
+#pragma unroll
+                                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                                    for (int r = 0; r < 4; ++r) {
+                                        const int row = i * 16 + 4 * fq + r;
+                                        if (row < rows) total[i][r] += set[(((o - 1) * wc_count + wc) * p.part_rows + row) * 16 + fi];
+                                    }
+                    }
+                    const int col = n0 + (b0 + b) * block_cols + fi;
+                    if (wk == 0 && col < p.n) {
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const int row = i * 16 + 4 * fq + r;
+                                if (row < rows) store_out(p.y, (size_t)(m0 + row) * p.n + col, total[i][r] * x_scale[i][r], p.y_type);
+                            }
                     }
                 }
-                // all reads of this stage have returned before it is refilled
-                wait_lgkmcnt0();
-                asm volatile("" ::: "memory");
-                __builtin_amdgcn_sched_barrier(0);
             }
-        }
-        // ---- the waves along K, added in wave order; register r of lane (fi, fq) holds y[16 i + 4 fq + r][n0 + fi]
-        if (p.wk > 1) {
-            __syncthreads();
-            v4f *part = reinterpret_cast<v4f *>(xs);
-            if (wk > 0)
-#pragma unroll
-                for (int i = 0; i < MT; ++i) part[(((wk - 1) * wc_count + wc) * MT + i) * 64 + lane] = total[i];
-            __syncthreads();
-            if (wk == 0)
-                for (int o = 1; o < p.wk; ++o)
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) total[i] += part[(((o - 1) * wc_count + wc) * MT + i) * 64 + lane];
-        }
-        if (wk == 0 && n0 + fi < p.n) {
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = i * 16 + 4 * fq + r;
-                    if (row < rows) {
-                        const float s = p.x_scale ? p.x_scale[m0 + row] : 1.0f;
-                        store_out(p.y, (size_t)(m0 + row) * p.n + n0 + fi, total[i][r] * s, p.y_type);
-                    }
-                }
         }
     }
 }

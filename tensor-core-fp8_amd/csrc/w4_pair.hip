@@ -1,0 +1,102 @@
+// Products with 4-bit weights, launch code of one pair of 16-bit type and way of expanding the weights.  Compiled five
+// times, with -DFP8GEMM_W4_F16=<0|1> (x and the expanded weights in bf16 or f16) -DFP8GEMM_W4_MODE=<kW4...> (w4_args.h).
+#include <algorithm>
+#include <cmath>
+
+#include "dispatch.h"
+#include "kernel_w4.h"
+
+#if !defined(FP8GEMM_W4_F16) || !defined(FP8GEMM_W4_MODE)
+#error "compile with -DFP8GEMM_W4_F16=<0|1> -DFP8GEMM_W4_MODE=<0|1|2>"
+#endif
+
+namespace fp8gemm_detail {
+
+template <bool F16, int MODE, int RUN, int MT, int KIND>
+struct W4KernelTag {};
+
+constexpr int kW4MaxLds = 160 * 1024;
+
+template <bool F16, int MODE, int RUN, int MT, int KIND>
+hipError_t launch_w4_kernel(W4Args p, hipStream_t s)
+{
+    // Rows of x that an expert has at a time, as far as the host can tell.
+    const int busy = std::min(p.rows, p.groups);
+    const int rows = std::min((p.rows + busy - 1) / busy, 16 * MT);
+    const long col_tiles = (p.n + 15) / 16, row_bytes = p.k / 2;
+    // How the eight waves are laid out, how many workgroups share a CU and how many blocks of columns each takes: the
+    // least time in units of one ring stage of a workgroup -- half a unit to add the waves along K up, six to
+    // start a pass, more to stage many rows of x, and two workgroups on a CU hide 15 % of each other's time.  (Two only
+    // where the registers of 16 waves fit.  MI355X, one row, us for the pick / the best of the eight layouts: 28672 x 8192 integers
+    // in runs of 128 27.1 / 27.1, of 32 43.9 / 36.5; 8192 x 8192 13.4 / 11.9; 4096 x 4096 7.9 / 7.9; 16 rows 28672 x 8192 42.5 / 42.8.)
+    constexpr int EB = w4_entry_bytes(MODE, KIND);
+    double best = 1e30;
+    int best_lds = 0;
+    p.part_rows = std::min(p.rows, 16 * MT);
+    for (int per_cu = MT == 1 ? 2 : 1; per_cu >= 1; --per_cu)
+        for (int wk = 1; wk <= kW4Waves; wk *= 2) {
+            if (wk > 1 && p.k <= (wk - 1) * kW4StageK) continue;
+            const int wc = kW4Waves / wk, unit = kW4StageK * wk, slot = w4_ring_bytes(1);
+            const long blocks = (col_tiles + wc - 1) / wc, whole = ((long)p.k + unit - 1) / unit * unit;
+            long each = std::min(blocks, (blocks * busy + 256 * per_cu - 1) / (256 * per_cu));
+            each = std::max(1L, std::min(each, ((1L << 31) - 1) / (16 * wc * row_bytes)));
+            const long x_bytes = rows * (whole * 2 + 16), block_bytes = (long)16 * wc * (((whole / RUN) * EB + 15) / 16 + 1) * 16;
+            const long fixed = w4_ring_bytes(kW4RingTwo) + w4_part_bytes(wk, p.part_rows);
+            const long room = kW4MaxLds / per_cu - fixed;
+            const long least = p.part_rows * w4_x_pitch(unit) + (long)16 * wc * (unit / RUN * EB + 31);
+            if (room < least) continue;
+            const bool fits = x_bytes + block_bytes <= room;
+            // (K in pieces: a pass for every block and piece)
+            const long at_once = fits ? std::min(each, (room - x_bytes) / block_bytes) : 1;
+            const double passes = fits ? (double)((each + at_once - 1) / at_once) : (double)each * (x_bytes + block_bytes) / room;
+            const double stages = (double)((p.k + unit - 1) / unit), staging = (fits ? 1.0 : (double)each) * rows * whole / 7000.0;
+            const long groups_of_waves = (blocks + each - 1) / each * busy, on_a_cu = (groups_of_waves + 255) / 256;
+            const double cost = (double)on_a_cu * (each * (stages + (wk > 1 ? 0.5 : 0.0)) + staging) * (on_a_cu > 1 && per_cu > 1 ? 0.85 : 1.0) +
+                                (double)((on_a_cu + per_cu - 1) / per_cu) * passes * 6.0;
+            if (cost < best) {
+                best = cost;
+                p.wk_shift = wk == 1 ? 0 : (wk == 2 ? 1 : (wk == 4 ? 2 : 3));
+                p.pass = fits ? (int)at_once : 0;
+                p.plan_rows = rows;
+                p.blocks = (int)each;
+                // (an expert may have more rows than the average: x gets the room that the CU has)
+                p.stage_bytes = (int)(p.groups > 1 || !fits ? room : std::max(least, x_bytes + at_once * block_bytes));
+                p.ring = room - p.stage_bytes >= (kW4RingFour - kW4RingTwo) * slot ? kW4RingFour : kW4RingTwo;
+                best_lds = (int)fixed + (p.ring - kW4RingTwo) * slot + p.stage_bytes;
+            }
+        }
+    if (best_lds == 0) return hipErrorInvalidValue;
+    const int lds = best_lds, wc = kW4Waves >> p.wk_shift;
+    auto kernel = gemv_w4_kernel<F16, MODE, RUN, MT, KIND>;
+    hipError_t e = allow_lds<W4KernelTag<F16, MODE, RUN, MT, KIND>>(kernel, kW4MaxLds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((col_tiles + wc * p.blocks - 1) / (wc * p.blocks)), (unsigned)p.groups), dim3(64 * kW4Waves), lds, s, p);
+    return hipGetLastError();
+}
+
+template <bool F16, int MODE, int RUN, int KIND>
+hipError_t launch_w4_rows(const W4Args &p, hipStream_t s)
+{
+    // rows of x per pass over the weights; with experts, what an expert has on average
+    const int average = (p.rows + p.groups - 1) / p.groups;
+    if (p.rows <= 16 || average <= 8) return launch_w4_kernel<F16, MODE, RUN, 1, KIND>(p, s);
+    if (p.rows <= 32 || average <= 16) return launch_w4_kernel<F16, MODE, RUN, 2, KIND>(p, s);
+    return launch_w4_kernel<F16, MODE, RUN, 4, KIND>(p, s);
+}
+
+template <bool F16, int MODE>
+hipError_t launch_w4(const W4Args &p, hipStream_t s)
+{
+    const bool long_runs = p.run % 128 == 0;
+    if constexpr (MODE == kW4Fp4Scaled) {
+        return long_runs ? launch_w4_rows<F16, MODE, 128, kW4ScaleByte>(p, s) : launch_w4_rows<F16, MODE, 32, kW4ScaleByte>(p, s);
+    } else {
+        if (p.scale_type == FP8GEMM_T_F32) return long_runs ? launch_w4_rows<F16, MODE, 128, kW4ScaleF32>(p, s) : launch_w4_rows<F16, MODE, 32, kW4ScaleF32>(p, s);
+        if (p.scale_type == FP8GEMM_T_F16) return long_runs ? launch_w4_rows<F16, MODE, 128, kW4ScaleF16>(p, s) : launch_w4_rows<F16, MODE, 32, kW4ScaleF16>(p, s);
+        return long_runs ? launch_w4_rows<F16, MODE, 128, kW4ScaleBf16>(p, s) : launch_w4_rows<F16, MODE, 32, kW4ScaleBf16>(p, s);
+    }
+}
+
+template hipError_t launch_w4<FP8GEMM_W4_F16 != 0, FP8GEMM_W4_MODE>(const W4Args &, hipStream_t);
+
+}  // namespace fp8gemm_detail
