@@ -168,10 +168,10 @@ hipError_t launch_quantize_columns(const GroupSpec &grp, int cols, const void *x
     const long grid = col_blocks * (grp.groups + 1);
     if (grid > 0x7FFFFFFFL) return hipErrorInvalidValue;
     if (vec)
-        hipLaunchKernelGGL((quantize_columns_kernel<TYPE, FMT, true>), dim3((unsigned)grid), dim3(256), 0, s, grp, cols, x, stride, x_rows, index, codes, ld,
+        hipLaunchKernelGGL((quantize_columns_kernel<TYPE, FMT, true>), dim3((unsigned)grid), dim3(kColThreads), 0, s, grp, cols, x, stride, x_rows, index, codes, ld,
                            scales);
     else
-        hipLaunchKernelGGL((quantize_columns_kernel<TYPE, FMT, false>), dim3((unsigned)grid), dim3(256), 0, s, grp, cols, x, stride, x_rows, index, codes, ld,
+        hipLaunchKernelGGL((quantize_columns_kernel<TYPE, FMT, false>), dim3((unsigned)grid), dim3(kColThreads), 0, s, grp, cols, x, stride, x_rows, index, codes, ld,
                            scales);
     return hipGetLastError();
 }

@@ -50,31 +50,46 @@ __device__ __forceinline__ uint32_t quant_four(float a, float b, float c, float 
     return w;
 }
 
-// eight consecutive elements from a 16-byte aligned place
+// eight consecutive elements as they are stored (a 16-bit type fills the first half)
+struct QuantRaw {
+    v4i lo, hi;
+};
+template <int TYPE>
+__device__ __forceinline__ QuantRaw quant_load8_raw(const void *base, size_t index)      // from a 16-byte aligned place
+{
+    QuantRaw r = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    if (TYPE == FP8GEMM_DEV_OUT_F32) {
+        const v4i *p = reinterpret_cast<const v4i *>(static_cast<const float *>(base) + index);
+        r.lo = p[0];
+        r.hi = p[1];
+    } else {
+        r.lo = *reinterpret_cast<const v4i *>(static_cast<const unsigned short *>(base) + index);
+    }
+    return r;
+}
+template <int TYPE>
+__device__ __forceinline__ void quant_unpack8(const QuantRaw &r, float v[8])
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = (uint32_t)r.lo[i], hi = (uint32_t)r.hi[i];
+        if (TYPE == FP8GEMM_DEV_OUT_F32) {
+            v[i] = __builtin_bit_cast(float, lo);
+            v[4 + i] = __builtin_bit_cast(float, hi);
+        } else if (TYPE == FP8GEMM_DEV_OUT_BF16) {
+            v[2 * i] = __builtin_bit_cast(float, lo << 16);
+            v[2 * i + 1] = __builtin_bit_cast(float, lo & 0xFFFF0000u);
+        } else {
+            v[2 * i] = (float)__builtin_bit_cast(_Float16, (unsigned short)(lo & 0xFFFFu));
+            v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(lo >> 16));
+        }
+    }
+}
 template <int TYPE>
 __device__ __forceinline__ void quant_load8(const void *base, size_t index, float v[8])
 {
-    if (TYPE == FP8GEMM_DEV_OUT_F32) {
-        const v4f *p = reinterpret_cast<const v4f *>(static_cast<const float *>(base) + index);
-        const v4f a = p[0], b = p[1];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = a[i];
-            v[4 + i] = b[i];
-        }
-    } else {
-        const v4i w = *reinterpret_cast<const v4i *>(static_cast<const unsigned short *>(base) + index);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (TYPE == FP8GEMM_DEV_OUT_BF16) {
-                v[2 * i] = __builtin_bit_cast(float, (uint32_t)w[i] << 16);
-                v[2 * i + 1] = __builtin_bit_cast(float, (uint32_t)w[i] & 0xFFFF0000u);
-            } else {
-                v[2 * i] = (float)__builtin_bit_cast(_Float16, (unsigned short)((uint32_t)w[i] & 0xFFFFu));
-                v[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)((uint32_t)w[i] >> 16));
-            }
-        }
-    }
+    const QuantRaw r = quant_load8_raw<TYPE>(base, index);
+    quant_unpack8<TYPE>(r, v);
 }
 
 // folds |x| into the running maximum of finite magnitudes; whether x is an infinity or a NaN
@@ -194,108 +209,147 @@ __global__ __launch_bounds__(256) void quantize_rows_any_kernel(int cols, const 
 
 // ---- transposed, grouped -------------------------------------------------------------------
 // codes_t (cols x ld): the tokens of group g, a column each, from its first run of kTokenRun columns on (group_table.h), zeros
-// behind its last token and behind the last group; scales (groups x cols).  A workgroup takes kColBlock columns
-// of one group, reads them twice (once for the maxima), and turns 128 x 64 pieces around in LDS so that every
-// column's 128 codes leave as one whole line.
+// behind its last token and behind the last group; scales (groups x cols).  HBM bound.  A workgroup takes kColBlock
+// columns (a line of 16-bit numbers) of one group, 256 or 512 rows at a time, quads of rows of eight columns a thread: a first walk
+// finds the maxima, the second one goes backwards, so that it starts with the rows that are still in registers (all of
+// them, for a group of no more rows) and goes on with those that are still cached.  128 x 64 pieces are turned
+// around in LDS, so that every column's 128 codes leave as one whole line.
 constexpr int kColBlock = 64;
+constexpr int kColThreads = 512;
+// rows at a time: four or eight a thread, which are 32 registers of either
+__host__ __device__ constexpr int col_rows(int type) { return kColThreads / 8 * (type == FP8GEMM_DEV_OUT_F32 ? 4 : 8); }
 constexpr int kColPitch = kTokenRun + 4;       // bytes of a column in LDS: 33 words, so that eight columns x eight words hit 64 banks
 
+// elements at + c .. at + c + 7, those from `cols` on as zeros
 template <int TYPE, bool VEC>
-__device__ __forceinline__ void quant_load_cols(const void *x, size_t at, int c, int cols, float v[8])
+__device__ __forceinline__ QuantRaw quant_load_cols(const void *x, size_t at, int c, int cols)
 {
+    QuantRaw r = {{0, 0, 0, 0}, {0, 0, 0, 0}};
     if (VEC) {
-        if (c < cols) {
-            quant_load8<TYPE>(x, at + c, v);
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+        if (c < cols) r = quant_load8_raw<TYPE>(x, at + c);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? load_in(x, at + c + i, TYPE) : 0.0f;
+        for (int i = 0; i < 8; ++i) {
+            if (c + i >= cols) continue;
+            if (TYPE == FP8GEMM_DEV_OUT_F32) {
+                const int w = static_cast<const int *>(x)[at + c + i];
+                if (i < 4)
+                    r.lo[i & 3] = w;
+                else
+                    r.hi[i & 3] = w;
+            } else {
+                const uint32_t h = static_cast<const unsigned short *>(x)[at + c + i];
+                r.lo[i / 2] = (int)((uint32_t)r.lo[i / 2] | (h << (16 * (i & 1))));
+            }
+        }
     }
+    return r;
 }
 
 template <int TYPE, int FMT, bool VEC>
-__global__ __launch_bounds__(256) void quantize_columns_kernel(GroupSpec grp, int cols, const void *__restrict__ x, size_t x_stride, int x_rows,
-                                                               const int *__restrict__ row_index, uint8_t *__restrict__ codes_t, size_t ld,
-                                                               float *__restrict__ scales)
+__global__ __launch_bounds__(kColThreads) void quantize_columns_kernel(GroupSpec grp, int cols, const void *__restrict__ x, size_t x_stride, int x_rows,
+                                                                       const int *__restrict__ row_index, uint8_t *__restrict__ codes_t, size_t ld,
+                                                                       float *__restrict__ scales)
 {
     using lds_int = __attribute__((address_space(3))) int;
+    constexpr int WAVES = kColThreads / 64, ROWS = col_rows(TYPE), RUNS = ROWS / kTokenRun, QUADS = ROWS / (kColThreads / 2);
     __shared__ int table[2 * (kMaxGroups + 1)];
-    __shared__ uint32_t amax_of[32][kColBlock];
-    __shared__ uint8_t turn[kColBlock * kColPitch];
+    __shared__ uint32_t amax_of[WAVES][kColBlock];
+    __shared__ uint8_t turn[RUNS][kColBlock * kColPitch];
     lds_int *tab_run = (lds_int *)table, *tab_row = (lds_int *)table + kMaxGroups + 1;
     build_group_table<kTokenRun>(grp, 0, 1, tab_run, tab_row);
     const int col_blocks = (cols + kColBlock - 1) / kColBlock;
     const int g = (int)(blockIdx.x / (unsigned)col_blocks);
     const int c0 = (int)(blockIdx.x % (unsigned)col_blocks) * kColBlock;
-    const int cc = threadIdx.x & 7, slot = threadIdx.x >> 3;       // eight columns, one of 32 rows
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int cc = threadIdx.x & 7, slot = threadIdx.x >> 3;       // eight columns, four of the rows
     const int c = c0 + cc * 8;
-    // the place of 16 codes in the write-out: column, piece
-    const int wcol = threadIdx.x >> 3, wpiece = threadIdx.x & 7;
+    // the place of 16 codes in the write-out: one of the runs written at once, column, piece of the run
+    constexpr int AT_ONCE = kColThreads / (8 * kColBlock);
+    const int wrun = threadIdx.x / (8 * kColBlock), wcol = (threadIdx.x >> 3) % kColBlock, wpiece = threadIdx.x & 7;
     if (g == grp.groups) {
         // behind the last group: zeros
-        for (size_t at = (size_t)tab_run[g] * kTokenRun; at < ld; at += kTokenRun)
-            for (int j = wcol; j < kColBlock; j += 32)
-                if (c0 + j < cols) *reinterpret_cast<v4i *>(codes_t + (size_t)(c0 + j) * ld + at + wpiece * 16) = v4i{0, 0, 0, 0};
+        for (size_t at = ((size_t)tab_run[g] + wrun) * kTokenRun; at < ld; at += AT_ONCE * kTokenRun)
+            if (c0 + wcol < cols) *reinterpret_cast<v4i *>(codes_t + (size_t)(c0 + wcol) * ld + at + wpiece * 16) = v4i{0, 0, 0, 0};
         return;
     }
     const int first = tab_row[g], end = tab_row[g + 1];
-    const auto source = [&](int r) -> long { return row_index ? (long)row_index[r] : (long)r; };
+    const int batches = end > first ? (end - first + ROWS - 1) / ROWS : 0;
+    QuantRaw raw[QUADS][4];
+    auto load = [&](int batch) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < QUADS; ++q) {
+            const int r0 = first + batch * ROWS + q * (kColThreads / 2) + slot * 4;
+            long src[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) src[u] = r0 + u < end ? (row_index ? (long)row_index[r0 + u] : (long)(r0 + u)) : -1;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                raw[q][u] = QuantRaw{{0, 0, 0, 0}, {0, 0, 0, 0}};
+                if (src[u] >= 0 && src[u] < x_rows) raw[q][u] = quant_load_cols<TYPE, VEC>(x, (size_t)src[u] * x_stride, c, cols);
+            }
+        }
+    };
     // ---- the columns' largest magnitudes
     uint32_t amax[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     bool odd = false;
-    for (int r = first + slot; r < end; r += 32) {
-        const long src = source(r);
-        if (src < 0 || src >= x_rows) continue;
-        float v[8];
-        quant_load_cols<TYPE, VEC>(x, (size_t)src * x_stride, c, cols, v);
+    for (int b = 0; b < batches; ++b) {
+        load(b);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) odd |= quant_fold(v[i], amax[i]);
+        for (int q = 0; q < QUADS; ++q)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                float v[8];
+                quant_unpack8<TYPE>(raw[q][u], v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) odd |= quant_fold(v[i], amax[i]);
+            }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax_of[slot][cc * 8 + i] = amax[i];
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int off = 8; off < 64; off <<= 1) {
+            const uint32_t o = (uint32_t)__shfl_xor((int)amax[i], off, 64);
+            amax[i] = o > amax[i] ? o : amax[i];
+        }
+        if (lane < 8) amax_of[wave][cc * 8 + i] = amax[i];
+    }
     const bool rough = __syncthreads_or(odd) != 0;
     float inv[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         uint32_t m = 0;
-        for (int s = 0; s < 32; ++s) {
-            const uint32_t o = amax_of[s][cc * 8 + i];
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const uint32_t o = amax_of[w][cc * 8 + i];
             m = o > m ? o : m;
         }
         const int e = quant_scale_exponent<FMT>(m);
         inv[i] = quant_inverse(e);
         if (slot == 0 && c + i < cols) scales[(size_t)g * cols + c + i] = quant_scale(e);
     }
-    // ---- the codes, a run of tokens at a time: a thread has four tokens of its eight columns
-    for (int r0 = first; r0 < end; r0 += kTokenRun) {
-        float v[4][8];
+    // ---- the codes
+    for (int b = batches - 1; b >= 0; --b) {
+        if (b < batches - 1) load(b);
+        __syncthreads();                                  // (the runs before have been written out)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int r = r0 + slot * 4 + u;
-            const long src = r < end ? source(r) : -1;
-            if (src >= 0 && src < x_rows) {
-                quant_load_cols<TYPE, VEC>(x, (size_t)src * x_stride, c, cols, v[u]);
-            } else {
+        for (int q = 0; q < QUADS; ++q) {
+            float v[4][8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[u][i] = 0.0f;
-            }
+            for (int u = 0; u < 4; ++u) quant_unpack8<TYPE>(raw[q][u], v[u]);
+            uint8_t *to = turn[q * (kColThreads / 256) + slot / 32] + cc * 8 * kColPitch + slot % 32 * 4;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                *reinterpret_cast<uint32_t *>(to + i * kColPitch) = quant_four<FMT>(v[0][i] * inv[i], v[1][i] * inv[i], v[2][i] * inv[i], v[3][i] * inv[i], rough);
         }
-        __syncthreads();                                  // (the run before has been written out)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<uint32_t *>(turn + (cc * 8 + i) * kColPitch + slot * 4) =
-                quant_four<FMT>(v[0][i] * inv[i], v[1][i] * inv[i], v[2][i] * inv[i], v[3][i] * inv[i], rough);
         __syncthreads();
-        const size_t at = ((size_t)tab_run[g] + (size_t)(r0 - first) / kTokenRun) * kTokenRun;
 #pragma unroll
-        for (int j = wcol; j < kColBlock; j += 32)
-            if (c0 + j < cols) {
-                const uint32_t *p = reinterpret_cast<const uint32_t *>(turn + j * kColPitch + wpiece * 16);
-                *reinterpret_cast<v4i *>(codes_t + (size_t)(c0 + j) * ld + at + wpiece * 16) = v4i{(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
-            }
+        for (int run = wrun; run < RUNS; run += AT_ONCE) {
+            const int r = b * RUNS + run;                 // run of the group
+            if (first + r * kTokenRun >= end || c0 + wcol >= cols) continue;
+            const uint32_t *p = reinterpret_cast<const uint32_t *>(turn[run] + wcol * kColPitch + wpiece * 16);
+            *reinterpret_cast<v4i *>(codes_t + (size_t)(c0 + wcol) * ld + ((size_t)tab_run[g] + r) * kTokenRun + wpiece * 16) = v4i{(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
+        }
     }
 }
 
