@@ -249,7 +249,9 @@ __device__ __forceinline__ void store_out4_stream(void *base, size_t index, v4f 
 {
     if (type == FP8GEMM_DEV_OUT_F32) {
         FP8GEMM_GLOBAL v4f *p = (FP8GEMM_GLOBAL v4f *)((FP8GEMM_GLOBAL float *)base + index);
-        asm volatile("global_store_dwordx4 %0, %1, off nt" : : "v"(p), "v"(v) : "memory");
+        // (two wait states before the registers of the data may be written again: a store of more than 64 bits reads them late,
+        // and the compiler, which would see to it, does not know what the statement holds)
+        asm volatile("global_store_dwordx4 %0, %1, off nt\n\ts_nop 1" : : "v"(p), "v"(v) : "memory");
     } else {
         FP8GEMM_GLOBAL v2u *p = (FP8GEMM_GLOBAL v2u *)((FP8GEMM_GLOBAL unsigned short *)base + index);
         const v2u w = out_pack4(v, type);
