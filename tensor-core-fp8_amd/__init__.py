@@ -420,39 +420,58 @@ T_F32, T_BF16, T_F16, T_E4M3, T_E5M2, T_E8M0 = 0, 1, 2, 3, 4, 5
 # checks below are written to cost a few microseconds.)
 
 
-def _wide_code(dtype):
+_torch = None        # the torch module and its type codes, looked up once
+_WIDE = {}
+_FP8 = {}
+
+
+def _setup():
+    global _torch
     import torch
-    if dtype is torch.bfloat16:
-        return OUT_BF16
-    if dtype is torch.float32:
-        return OUT_F32
-    if dtype is torch.float16:
-        return OUT_F16
-    raise Fp8GemmError("expected float32, bfloat16 or float16, got %s" % dtype)
+    _WIDE.update({torch.float32: OUT_F32, torch.bfloat16: OUT_BF16, torch.float16: OUT_F16})
+    _FP8.update({E4M3: torch.float8_e4m3fn, E5M2: torch.float8_e5m2, torch.float8_e4m3fn: E4M3, torch.float8_e5m2: E5M2})
+    _torch = torch
+    return lib()
+
+
+def _wide_code(dtype):
+    code = _WIDE.get(dtype)
+    if code is None:
+        raise Fp8GemmError("expected float32, bfloat16 or float16, got %s" % dtype)
+    return code
+
+
+def _fp8_code(t, fmt):
+    """Format of an operand of codes, or as given for codes held in bytes."""
+    code = _FP8.get(t.dtype)
+    if code is None:
+        if fmt not in (E4M3, E5M2) or t.dtype is not _torch.uint8:
+            raise Fp8GemmError("operand must be float8_e4m3fn / float8_e5m2, or uint8 with an explicit format")
+        code = fmt
+    return code
 
 
 def _device_of(first, *others):
-    """The device of the operands, which have to share one."""
-    device = first.device
-    if device.type != "cuda":
+    """Index of the device that the operands share."""
+    index = first.get_device()
+    if index < 0:
         raise Fp8GemmError("operands must live in device memory")
     for t in others:
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             raise Fp8GemmError("operands must live in the memory of one device")
-    return device
+    return index
 
 
-def _launch(fn, device, stream, *args):
+def _launch(fn, index, stream, *args):
     """fn(*args, stream) with the operands' device current (the library launches on the current one); the
     stream defaults to that device's current stream."""
-    import torch
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            return _launch(fn, device, stream, *args)
+    if _torch._C._cuda_getDevice() != index:
+        with _torch.cuda.device(index):
+            return _launch(fn, index, stream, *args)
     if stream is None:
-        handle = torch._C._cuda_getCurrentRawStream(device.index)
+        handle = _torch._C._cuda_getCurrentRawStream(index)
     else:
-        if stream.device != device:
+        if stream.device.index != index:
             raise Fp8GemmError("the stream belongs to another device than the operands")
         handle = stream.cuda_stream
     code = fn(*args, handle)
@@ -462,25 +481,29 @@ def _launch(fn, device, stream, *args):
 
 def _floats(t, count, what):
     """Pointer to `count` contiguous float32 device elements, or None."""
-    import torch
     if t is None:
         return None
-    if t.dtype is not torch.float32 or t.numel() != count or not t.is_contiguous():
+    if t.dtype is not _torch.float32 or t.numel() != count or not t.is_contiguous():
         raise Fp8GemmError("%s: expected %d contiguous float32 elements" % (what, count))
+    return t.data_ptr()
+
+
+def _ints(t, what):
+    if t.dtype is not _torch.int32 or not t.is_contiguous():
+        raise Fp8GemmError("%s: expected contiguous int32 elements" % what)
     return t.data_ptr()
 
 
 def _offsets(t):
     if t.dim() != 1 or t.shape[0] < 2:
         raise Fp8GemmError("row_offsets holds one more element than there are experts")
-    return _dev_ints(t), t.shape[0] - 1
+    return _ints(t, "row_offsets"), t.shape[0] - 1
 
 
-def _output(out, shape, dtype, device):
-    import torch
+def _output(out, shape, dtype, like):
     if out is None:
-        return torch.empty(shape, dtype=dtype or torch.float32, device=device)
-    if tuple(out.shape) != shape or not out.is_contiguous() or (dtype is not None and out.dtype != dtype):
+        return like.new_empty(shape, dtype=dtype or _torch.float32)
+    if out.shape != shape or not out.is_contiguous() or (dtype is not None and out.dtype != dtype):
         raise Fp8GemmError("out must be a contiguous %s tensor of the wanted type" % (shape,))
     return out
 
@@ -502,25 +525,22 @@ def _wide_matrix(x, row_index):
 
 
 def _fp8_dtype(fmt):
-    import torch
-    if fmt == E4M3:
-        return torch.float8_e4m3fn
-    if fmt == E5M2:
-        return torch.float8_e5m2
-    raise Fp8GemmError("fmt is E4M3 or E5M2")
+    if fmt not in (E4M3, E5M2):
+        raise Fp8GemmError("fmt is E4M3 or E5M2")
+    return _FP8[fmt]
 
 
 def quantize_rows(x, fmt=E4M3, row_index=None, codes=None, scales=None, stream=None):
     """(codes, scales) of the rows of x (float32 / bfloat16 / float16, unit column stride), or of the rows
     row_index (int32) names (an index outside x: a row of zeros): codes (rows, cols) float8, scales (rows,)
     float32 powers of two, x ~ codes * scales[:, None].  Through fp8gemm_quantize_rows."""
-    import torch
+    L = _setup() if _torch is None else lib()
     rows, x_rows, cols, x_type, stride = _wide_matrix(x, row_index)
     device = _device_of(x, row_index, codes, scales)
-    codes = _output(codes, (rows, cols), _fp8_dtype(fmt), device)
-    scales = _output(scales, (rows,), torch.float32, device)
-    _launch(lib().fp8gemm_quantize_rows, device, stream, rows, cols, x.data_ptr(), x_type, stride, x_rows,
-            None if row_index is None else _dev_ints(row_index), fmt, codes.data_ptr(), scales.data_ptr())
+    codes = _output(codes, (rows, cols), _fp8_dtype(fmt), x)
+    scales = _output(scales, (rows,), _torch.float32, x)
+    _launch(L.fp8gemm_quantize_rows, device, stream, rows, cols, x.data_ptr(), x_type, stride, x_rows,
+            None if row_index is None else _ints(row_index, "row_index"), fmt, codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
 
@@ -528,15 +548,15 @@ def quantize_columns(x, row_offsets, fmt=E4M3, row_index=None, codes=None, scale
     """(codes, scales) of x transposed, for gemm_grouped_wgrad: codes (cols, grouped_ld(rows, groups)) float8,
     every expert's tokens in whole runs of 128 columns with zeros behind them, scales (groups, cols).
     row_index as in quantize_rows.  Through fp8gemm_quantize_columns."""
-    import torch
+    L = _setup() if _torch is None else lib()
     rows, x_rows, cols, x_type, stride = _wide_matrix(x, row_index)
     device = _device_of(x, row_offsets, row_index, codes, scales)
     offs, groups = _offsets(row_offsets)
     ld = grouped_ld(rows, groups)
-    codes = _output(codes, (cols, ld), _fp8_dtype(fmt), device)
-    scales = _output(scales, (groups, cols), torch.float32, device)
-    _launch(lib().fp8gemm_quantize_columns, device, stream, groups, rows, cols, offs, x.data_ptr(), x_type, stride, x_rows,
-            None if row_index is None else _dev_ints(row_index), fmt, codes.data_ptr(), ld, scales.data_ptr())
+    codes = _output(codes, (cols, ld), _fp8_dtype(fmt), x)
+    scales = _output(scales, (groups, cols), _torch.float32, x)
+    _launch(L.fp8gemm_quantize_columns, device, stream, groups, rows, cols, offs, x.data_ptr(), x_type, stride, x_rows,
+            None if row_index is None else _ints(row_index, "row_index"), fmt, codes.data_ptr(), ld, scales.data_ptr())
     return codes, scales
 
 
@@ -545,6 +565,7 @@ def gemm_grouped(a, b, row_offsets, a_scale=None, b_scale=None, out_dtype=None, 
     """out[i] = a_scale[i] * b_scale[g] * (a[i] . b[g]^T) for the rows i of every expert g: a (m, k), b (groups, n, k)
     codes, row_offsets (groups + 1,) int32, a_scale (m,), b_scale (groups, n) or (groups,) float32 or None.
     Rows outside the experts are left as they are (uninitialised when out is None).  Through fp8gemm_grouped."""
+    L = _setup() if _torch is None else lib()
     device = _device_of(a, b, row_offsets, a_scale, b_scale, out)
     if a.dim() != 2 or b.dim() != 3 or a.shape[1] != b.shape[2]:
         raise Fp8GemmError("a (m, k) and b (groups, n, k) do not fit")
@@ -554,10 +575,10 @@ def gemm_grouped(a, b, row_offsets, a_scale=None, b_scale=None, out_dtype=None, 
     if b.shape[0] != groups:
         raise Fp8GemmError("row_offsets is for %d experts, b holds %d" % (groups, b.shape[0]))
     (m, k), n = a.shape, b.shape[1]
-    out = _output(out, (m, n), out_dtype, device)
+    out = _output(out, (m, n), out_dtype, a)
     per_column = b_scale is not None and b_scale.dim() == 2
-    _launch(lib().fp8gemm_grouped_tuned, device, stream, groups, m, k, n, offs, a.data_ptr(), _fmt_of(a, a_fmt), b.data_ptr(),
-            _fmt_of(b, b_fmt), out.data_ptr(), _wide_code(out.dtype), _floats(a_scale, m, "a_scale"),
+    _launch(L.fp8gemm_grouped_tuned, device, stream, groups, m, k, n, offs, a.data_ptr(), _fp8_code(a, a_fmt), b.data_ptr(),
+            _fp8_code(b, b_fmt), out.data_ptr(), _wide_code(out.dtype), _floats(a_scale, m, "a_scale"),
             _floats(b_scale, groups * n if per_column else groups, "b_scale"), int(per_column), variant)
     return out
 
@@ -567,6 +588,7 @@ def gemm_grouped_wgrad(a_t, b_t, row_offsets, rows, a_scale=None, b_scale=None, 
     """out[g] = a_scale[g][:, None] * b_scale[g] * (a_t . b_t^T over the tokens of expert g): a_t (m, ld), b_t (n, ld) codes
     as quantize_columns lays them out for `rows` rows, a_scale (groups, m), b_scale (groups, n) float32 or None;
     out (groups, m, n), added to what it holds if accumulate.  Through fp8gemm_grouped_wgrad."""
+    L = _setup() if _torch is None else lib()
     device = _device_of(a_t, b_t, row_offsets, a_scale, b_scale, out)
     if a_t.dim() != 2 or b_t.dim() != 2 or a_t.shape[1] != b_t.shape[1]:
         raise Fp8GemmError("a_t (m, ld) and b_t (n, ld) do not fit")
@@ -576,9 +598,9 @@ def gemm_grouped_wgrad(a_t, b_t, row_offsets, rows, a_scale=None, b_scale=None, 
         raise Fp8GemmError("accumulate needs the tensor to add to")
     offs, groups = _offsets(row_offsets)
     (m, ld), n = a_t.shape, b_t.shape[0]
-    out = _output(out, (groups, m, n), out_dtype, device)
-    _launch(lib().fp8gemm_grouped_wgrad_tuned, device, stream, groups, rows, m, n, offs, a_t.data_ptr(), _fmt_of(a_t, a_fmt),
-            b_t.data_ptr(), _fmt_of(b_t, b_fmt), ld, out.data_ptr(), _wide_code(out.dtype), _floats(a_scale, groups * m, "a_scale"),
+    out = _output(out, (groups, m, n), out_dtype, a_t)
+    _launch(L.fp8gemm_grouped_wgrad_tuned, device, stream, groups, rows, m, n, offs, a_t.data_ptr(), _fp8_code(a_t, a_fmt),
+            b_t.data_ptr(), _fp8_code(b_t, b_fmt), ld, out.data_ptr(), _wide_code(out.dtype), _floats(a_scale, groups * m, "a_scale"),
             _floats(b_scale, groups * n, "b_scale"), int(bool(accumulate)), variant)
     return out
 
@@ -589,7 +611,8 @@ def gemv_w4(x, w, scales, run, w_fmt=W4_INT, zeros=None, x_scale=None, row_offse
     low nibbles), scales (n, k/run) float32 / bfloat16 / float16 or uint8 (powers of two, 127 = 1), zeros (n, k/run)
     uint8 or None, x_scale (m,) float32 or None.  With row_offsets (groups + 1,) the rows of x are sorted by expert and
     w, scales, zeros have a leading axis of experts.  Through fp8gemm_gemv_w4 / fp8gemm_grouped_w4."""
-    import torch
+    L = _setup() if _torch is None else lib()
+    torch = _torch
     device = _device_of(x, w, scales, zeros, x_scale, row_offsets, out)
     if x.dim() != 2 or not (x.is_contiguous() and w.is_contiguous()):
         raise Fp8GemmError("x must be a matrix, operands contiguous")
@@ -615,12 +638,12 @@ def gemv_w4(x, w, scales, run, w_fmt=W4_INT, zeros=None, x_scale=None, row_offse
     elif x.dtype is torch.float16:
         x_type = T_F16
     else:
-        x_type = T_E4M3 if _fmt_of(x, x_fmt) == E4M3 else T_E5M2
-    out = _output(out, (m, n), out_dtype, device)
+        x_type = T_E4M3 if _fp8_code(x, x_fmt) == E4M3 else T_E5M2
+    out = _output(out, (m, n), out_dtype, x)
     args = (m, k, n, x.data_ptr(), x_type, _floats(x_scale, m, "x_scale"), w.data_ptr(), w_fmt, run, scales.data_ptr(), scale_type,
             None if zeros is None else zeros.data_ptr(), out.data_ptr(), _wide_code(out.dtype))
     if offs is None:
-        _launch(lib().fp8gemm_gemv_w4, device, stream, *args)
+        _launch(L.fp8gemm_gemv_w4, device, stream, *args)
     else:
-        _launch(lib().fp8gemm_grouped_w4, device, stream, groups, m, k, n, offs, *args[3:])
+        _launch(L.fp8gemm_grouped_w4, device, stream, groups, m, k, n, offs, *args[3:])
     return out

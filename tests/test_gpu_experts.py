@@ -1,0 +1,156 @@
+"""The operators for layers with experts together, as a layer uses them: tokens gathered by expert and quantised, the product,
+the gradients of input and matrices, a decoding step on 4-bit matrices; eager, and captured into one HIP graph."""
+import zlib
+
+import pytest
+import torch
+
+from expert_util import codes, fp8_product, offsets_of, places, rounding, w4_values
+
+pytestmark = pytest.mark.gpu
+
+TOKENS, TOP, EXPERTS, K, N = 300, 2, 8, 256, 384
+
+
+def generator(*key):
+    return torch.Generator(device="cuda").manual_seed(zlib.crc32(repr(key).encode()))
+
+
+def route(gen, off, index):
+    """Two experts for every token: off (EXPERTS + 1) and index (TOKENS * TOP) are filled in place."""
+    want = torch.randn((TOKENS, EXPERTS), generator=gen, device="cuda") + torch.linspace(1, -1, EXPERTS, device="cuda")
+    expert = want.topk(TOP, dim=1).indices.flatten()
+    order = torch.argsort(expert, stable=True)
+    index.copy_((order // TOP).to(torch.int32))
+    off[1:] = torch.cumsum(torch.bincount(expert, minlength=EXPERTS), 0).to(torch.int32)
+
+
+class Layer:
+    """y = x W[expert]^T on quantised operands, and its gradients."""
+
+    def __init__(self, pkg, gen):
+        self.pkg = pkg
+        self.w = torch.randn((EXPERTS, N, K), generator=gen, device="cuda").to(torch.bfloat16)
+        flat = lambda t: pkg.quantize_rows(t.reshape(-1, t.shape[-1]).contiguous())  # noqa: E731
+        c, s = flat(self.w)
+        self.wq, self.ws = c.view(EXPERTS, N, K), s.view(EXPERTS, N)
+        c, s = flat(self.w.transpose(1, 2))
+        self.wtq, self.wts = c.view(EXPERTS, K, N), s.view(EXPERTS, K)
+
+    def step(self, x, dy, off, index):
+        pkg = self.pkg
+        xq, xs = pkg.quantize_rows(x, pkg.E4M3, row_index=index)
+        y = pkg.gemm_grouped(xq, self.wq, off, a_scale=xs, b_scale=self.ws, out_dtype=torch.bfloat16)
+        dyq, dys = pkg.quantize_rows(dy, pkg.E5M2)
+        dx = pkg.gemm_grouped(dyq, self.wtq, off, a_scale=dys, b_scale=self.wts, out_dtype=torch.bfloat16)
+        dyt, dyts = pkg.quantize_columns(dy, off, pkg.E5M2)
+        xt, xts = pkg.quantize_columns(x, off, pkg.E4M3, row_index=index)
+        dw = pkg.gemm_grouped_wgrad(dyt, xt, off, index.numel(), a_scale=dyts, b_scale=xts, out_dtype=torch.float32)
+        return {"xq": xq, "xs": xs, "y": y, "dyq": dyq, "dys": dys, "dx": dx, "dyt": dyt, "dyts": dyts, "xt": xt, "xts": xts, "dw": dw}
+
+
+def check_step(layer, off, r):
+    at, counts, _ = places(off.tolist(), TOKENS * TOP)
+    for g, c in enumerate(counts):
+        lo = int(off[g])
+        for a, sa, b, sb, out in ((r["xq"], r["xs"], layer.wq, layer.ws, r["y"]), (r["dyq"], r["dys"], layer.wtq, layer.wts, r["dx"])):
+            y, tol = fp8_product(a[lo:lo + c].double(), b[g].double())
+            f = sa[lo:lo + c, None].double() * sb[g].double()
+            assert ((out[lo:lo + c].double() - y * f).abs() <= tol * f + rounding(y * f, torch.bfloat16) * 1.0001).all()
+        y, tol = fp8_product(r["dyt"][:, at[g]:at[g] + c].double(), r["xt"][:, at[g]:at[g] + c].double())
+        f = r["dyts"][g][:, None].double() * r["xts"][g].double()
+        assert ((r["dw"][g].double() - y * f).abs() <= tol * f + rounding(y * f, torch.float32) * 1.0001).all()
+
+
+def test_layer_forward_and_gradients(pkg):
+    gen = generator("layer")
+    layer = Layer(pkg, gen)
+    x = torch.randn((TOKENS, K), generator=gen, device="cuda").to(torch.bfloat16)
+    dy = (0.01 * torch.randn((TOKENS * TOP, N), generator=gen, device="cuda")).to(torch.bfloat16)
+    off, index = torch.zeros(EXPERTS + 1, dtype=torch.int32, device="cuda"), torch.zeros(TOKENS * TOP, dtype=torch.int32, device="cuda")
+    route(gen, off, index)
+    r = layer.step(x, dy, off, index)
+    check_step(layer, off, r)
+    # the matrices' gradient against differences: the loss sum(dy * y) on the operands that the gradient saw, along a
+    # random direction; it is linear in the matrices, so the difference is the derivative up to the products' tolerance
+    at, counts, _ = places(off.tolist(), TOKENS * TOP)
+    for g, c in enumerate(counts):
+        a = r["dyt"][:, at[g]:at[g] + c].double() * r["dyts"][g][:, None].double()
+        b = r["xt"][:, at[g]:at[g] + c].double() * r["xts"][g][:, None].double()
+        d = torch.randn((N, K), generator=gen, device="cuda").double()
+        loss = lambda w: (a.t().contiguous() * (b.t().contiguous() @ w.t().contiguous())).sum()  # noqa: E731
+        w = layer.w[g].double()
+        diff = (loss(w + 0.5 * d) - loss(w - 0.5 * d))
+        _, tol = fp8_product(r["dyt"][:, at[g]:at[g] + c].double(), r["xt"][:, at[g]:at[g] + c].double())
+        tol = tol * r["dyts"][g][:, None].double() * r["xts"][g].double() + r["dw"][g].double().abs() * 2.0 ** -23
+        # (64-bit rounding of the two losses: their terms are at most ~1e5 in sum)
+        assert (diff - (r["dw"][g].double() * d).sum()).abs() <= (tol * d.abs()).sum() + 1e-9
+
+
+def test_layer_captured_and_replayed_with_other_routes(pkg):
+    gen = generator("graph")
+    layer = Layer(pkg, gen)
+    x = torch.randn((TOKENS, K), generator=gen, device="cuda").to(torch.bfloat16)
+    dy = torch.randn((TOKENS * TOP, N), generator=gen, device="cuda").to(torch.bfloat16)
+    off, index = torch.zeros(EXPERTS + 1, dtype=torch.int32, device="cuda"), torch.zeros(TOKENS * TOP, dtype=torch.int32, device="cuda")
+    route(gen, off, index)
+    layer.step(x, dy, off, index)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        r = layer.step(x, dy, off, index)
+    for _ in range(4):
+        x.copy_(torch.randn((TOKENS, K), generator=gen, device="cuda"))
+        route(gen, off, index)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = layer.step(x, dy, off, index)
+        for key in r:
+            same = r[key].view(torch.uint8) if r[key].element_size() == 1 else r[key]
+            assert torch.equal(same, eager[key].view(same.dtype) if same.dtype == torch.uint8 else eager[key]), key
+
+
+def test_decoding_step_in_four_bits(pkg):
+    """Hidden state to codes, gathered for its experts, through 4-bit matrices."""
+    gen = generator("decode")
+    run = 32
+    w = torch.randint(0, 256, (EXPERTS, N, K // 2), generator=gen, dtype=torch.uint8, device="cuda")
+    s = torch.randint(120, 128, (EXPERTS, N, K // run), generator=gen, dtype=torch.uint8, device="cuda")
+    h = torch.randn((3, K), generator=gen, device="cuda").to(torch.bfloat16)
+    index = torch.tensor([2, 0, 1, 0, 2, 1], dtype=torch.int32, device="cuda")
+    off = offsets_of([1, 0, 2, 0, 0, 3, 0, 0])
+    xq, xs = pkg.quantize_rows(h, pkg.E4M3, row_index=index)
+    for x, scale in ((xq, xs), (h[index.long()].contiguous(), None)):
+        y = pkg.gemv_w4(x, w, s, run, w_fmt=pkg.W4_E2M1, x_scale=scale, row_offsets=off, out_dtype=torch.bfloat16)
+        xd = x.double() * (1.0 if scale is None else scale[:, None].double())
+        for g in range(EXPERTS):
+            lo, hi = int(off[g]), int(off[g + 1])
+            if hi > lo:
+                v = w4_values(w[g], s[g], run, 1)
+                ref = xd[lo:hi] @ v.t().contiguous()
+                tol = 2 * K * 2.0 ** -24 * (xd[lo:hi].abs() @ v.abs().t().contiguous()) + rounding(ref, torch.bfloat16) * 1.0001
+                assert ((y[lo:hi].double() - ref).abs() <= tol).all()
+
+
+def test_operands_on_another_stream_and_wrong_places(pkg):
+    """Launches go to the current stream, or the one named; operands of two kinds of memory are refused."""
+    gen = generator("streams")
+    a, b = codes(gen, (64, 128), 0), codes(gen, (2, 64, 128), 0)
+    off = offsets_of([30, 34])
+    want = pkg.gemm_grouped(a, b, off)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = pkg.gemm_grouped(a, b, off)
+    named = pkg.gemm_grouped(a, b, off, stream=side)
+    side.synchronize()
+    assert torch.equal(want, got) and torch.equal(want, named)
+    for bad in (lambda: pkg.gemm_grouped(a, b, off.cpu()), lambda: pkg.gemm_grouped(a, b.cpu(), off), lambda: pkg.gemm_grouped(a, b, off.long()), lambda: pkg.gemm_grouped(a[:, :64], b, off),
+                lambda: pkg.gemm_grouped(a.t(), b, off), lambda: pkg.gemm_grouped(a, b, off[:2]), lambda: pkg.gemm_grouped(a, b, off, a_scale=torch.ones(63, device="cuda")),
+                lambda: pkg.gemm_grouped(a, b, off, out=torch.empty(64, 65, device="cuda")), lambda: pkg.gemm_grouped(a, b, off, out_dtype=torch.float64),
+                lambda: pkg.quantize_rows(torch.zeros(4, 8, device="cuda", dtype=torch.float64)), lambda: pkg.quantize_rows(torch.zeros(8, device="cuda").expand(4, 8)),
+                lambda: pkg.quantize_rows(torch.zeros(4, 8, device="cuda"), fmt=7), lambda: pkg.gemm_grouped_wgrad(a, a, off, 64), lambda: pkg.gemm_grouped_wgrad(a, a, off, 64, accumulate=True),
+                lambda: pkg.gemv_w4(a.to(torch.bfloat16), b.view(torch.uint8)[0], torch.ones(64, 4, device="cuda"), 32),
+                lambda: pkg.gemv_w4(a.to(torch.bfloat16), b.view(torch.uint8)[0, :, :64].contiguous(), torch.ones(64, 3, device="cuda"), 32)):
+        with pytest.raises((pkg.Fp8GemmError, TypeError)):
+            bad()

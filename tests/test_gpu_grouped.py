@@ -207,6 +207,34 @@ def test_grouped_on_two_streams_at_once(pkg):
     assert all(torch.equal(o, ref) for o in outs)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_grouped_output_anywhere(pkg, dtype):
+    """Results that do not start on 16 bytes; what lies around them stays."""
+    gen = generator("place")
+    off, a, b = case(gen, [40, 0, 25], 256, 132, 0, 0)
+    for variant in ROWS_VARIANTS:
+        for shift in (1, 2, 5):
+            store = torch.full((65 * 132 + 16,), 3.0, dtype=dtype, device="cuda")
+            out = store[shift:shift + 65 * 132].view(65, 132)
+            pkg.gemm_grouped(a, b, off, out=out, variant=variant)
+            check_rows(out, off, a, b, None, None, dtype)
+            assert (store[:shift] == 3.0).all() and (store[shift + 65 * 132:] == 3.0).all()
+
+
+def test_grouped_many_experts(pkg):
+    """The largest number of experts, most of them without rows, rows in the first and the last."""
+    gen = generator("1024")
+    counts = [0] * 1024
+    for g, c in ((0, 3), (1, 1), (63, 2), (64, 70), (500, 1), (1022, 5), (1023, 130)):
+        counts[g] = c
+    off = offsets_of(counts)
+    m = sum(counts)
+    a, b = codes(gen, (m, 256), 0), codes(gen, (1024, 64, 256), 0)
+    for variant in ROWS_VARIANTS:
+        out = pkg.gemm_grouped(a, b, off, out_dtype=torch.float32, variant=variant)
+        check_rows(out, off, a, b, None, None, torch.float32)
+
+
 # ---------------------------------------------------------------- weight gradient
 def transposed(gen, counts, m, fmt, extra=0):
     """(m, ld) codes with every expert's tokens in whole runs of 128, zeros behind them; NaN codes where nothing may be read."""
@@ -318,3 +346,36 @@ def test_wgrad_operands_that_end_with_their_memory(pkg):
         y, tol = fp8_product(a.float()[pick].double(), b.double())
         for variant in (13, 18):
             check(pkg.gemm_grouped_wgrad(a, b, one, rows, variant=variant)[0][pick], y, tol + rounding(y, torch.float32) * 1.0001)
+
+
+def test_wgrad_many_experts_and_results_beyond_31_bits(pkg):
+    gen = generator("wgrad many")
+    counts = [0] * 1024
+    for g, c in ((0, 3), (64, 129), (1023, 7)):
+        counts[g] = c
+    off, a, at, cs = transposed(gen, counts, 2048, 0)
+    _, b, _, _ = transposed(gen, counts, 1152, 0)
+    for variant in (13, 18):
+        out = torch.full((1024, 2048, 1152), 5.0, dtype=torch.bfloat16, device="cuda")
+        assert out.numel() > 2 ** 31
+        pkg.gemm_grouped_wgrad(a, b, off, sum(counts), out=out, variant=variant)
+        for g in (0, 64, 1023):
+            y, tol = fp8_product(a[-64:, at[g]:at[g] + cs[g]].double(), b[-100:, at[g]:at[g] + cs[g]].double())
+            check(out[g, -64:, -100:], y, tol + rounding(y, torch.bfloat16) * 1.0001)
+        for g in (1, 63, 500, 1022):
+            assert not out[g].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_wgrad_output_anywhere(pkg, dtype):
+    gen = generator("wgrad place")
+    off, a, at, cs = transposed(gen, [100, 0, 30], 130, 0)
+    _, b, _, _ = transposed(gen, [100, 0, 30], 68, 0)
+    size = 3 * 130 * 68
+    for variant in (13, 18):
+        for shift in (1, 3):
+            store = torch.full((size + 16,), 3.0, dtype=dtype, device="cuda")
+            out = store[shift:shift + size].view(3, 130, 68)
+            pkg.gemm_grouped_wgrad(a, b, off, 130, out=out, variant=variant)
+            check_wgrad(out, at, cs, a, b, None, None, dtype)
+            assert (store[:shift] == 3.0).all() and (store[shift + size:] == 3.0).all()

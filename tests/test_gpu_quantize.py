@@ -149,6 +149,42 @@ def test_columns_gathered_strided_and_rows_outside(pkg):
         check_columns(pkg, x, [10, 3, 20], 1, first=7)               # rows in front of the first and behind the last expert
 
 
+def test_smallest_numbers(pkg):
+    """Subnormal fp32 and fp16: scales stop at 2^-126."""
+    x = torch.zeros((4, 72), device="cuda")
+    x[0, 3], x[0, 4] = 1e-40, -3e-41
+    x[1, 0], x[1, 71] = 2.0 ** -149, 2.0 ** -126
+    x[2, 5] = 2.0 ** -126 * 448
+    x[3, 5] = 2.0 ** -120
+    for fmt in (0, 1):
+        v, s = quantized(x, fmt, 1)
+        got, scales = pkg.quantize_rows(x, fmt)
+        assert torch.equal(scales.double(), s)
+        same(got, v)
+        check_columns(pkg, x, [2, 2], fmt)
+    h = torch.zeros((2, 64), device="cuda", dtype=torch.float16)
+    h[0, 1], h[0, 2], h[1, 63] = 6e-8, -3e-7, 6e-8
+    v, s = quantized(h, 0, 1)
+    got, scales = pkg.quantize_rows(h)
+    assert torch.equal(scales.double(), s)
+    same(got, v)
+
+
+def test_columns_of_many_experts(pkg):
+    gen = generator("1024")
+    counts = [0] * 1024
+    for g, c in ((0, 3), (1, 1), (64, 600), (1022, 5), (1023, 130)):
+        counts[g] = c
+    check_columns(pkg, wide(gen, sum(counts), 200, torch.bfloat16), counts, 0)
+
+
+def test_long_experts(pkg):
+    """More rows of one expert than a workgroup holds at a time, several times over."""
+    gen = generator("long")
+    for dtype in WIDE:
+        check_columns(pkg, wide(gen, 3000, 136, dtype), [1, 2500, 0, 499], 1)
+
+
 def test_calls_captured_and_replayed(pkg):
     gen = generator("graph")
     x = wide(gen, 256, 512, torch.bfloat16)

@@ -147,6 +147,58 @@ def test_experts(pkg, counts, w_fmt, run, scale):
     assert (y[:2] == 9.0).all() and (y[int(off[-1]):] == 9.0).all()
 
 
+def test_many_experts_and_results_anywhere(pkg):
+    gen = generator("1024")
+    counts = [0] * 1024
+    for g, c in ((0, 3), (1, 1), (500, 40), (1023, 2)):
+        counts[g] = c
+    n, k, run = 40, 256, 64
+    w, s, z = weights(gen, (1024,), n, k, run, 0, torch.float16, True)
+    off = offsets_of(counts)
+    m = sum(counts)
+    x = torch.randn((m, k), generator=gen, device="cuda").to(torch.float16)
+    for dtype in (torch.float32, torch.bfloat16):
+        store = torch.full((m * n + 9,), 3.0, dtype=dtype, device="cuda")
+        y = store[3:3 + m * n].view(m, n)
+        pkg.gemv_w4(x, w, s, run, zeros=z, row_offsets=off, out=y)
+        for g in (0, 1, 500, 1023):
+            lo, hi = int(off[g]), int(off[g + 1])
+            ref = x[lo:hi].double() @ w4_values(w[g], s[g], run, 0, z[g]).t().contiguous()
+            bound = 62.0 * s[g].double().repeat_interleave(run, -1)
+            assert ((y[lo:hi].double() - ref).abs() <= tolerance(x[lo:hi].double(), None, bound, dtype, ref)).all()
+        assert (store[:3] == 3.0).all() and (store[3 + m * n:] == 3.0).all()
+
+
+def test_experts_with_more_rows_than_the_average(pkg):
+    """One expert has nearly all rows: x is staged in pieces where the plan had it whole."""
+    gen = generator("skew")
+    for n, k, run, w_fmt, scale, x_type in ((96, 8192, 128, 0, torch.float16, torch.bfloat16), (4096, 4096, 32, 1, torch.uint8, torch.bfloat16), (96, 28672, 128, 1, torch.float32, torch.float16)):
+        counts = [0, 1, 61, 0, 2, 0, 0, 0]
+        w, s, z = weights(gen, (8,), n, k, run, w_fmt, scale, w_fmt == 0)
+        off = offsets_of(counts)
+        x = torch.randn((64, k), generator=gen, device="cuda").to(x_type)
+        y = pkg.gemv_w4(x, w, s, run, w_fmt=w_fmt, zeros=z, row_offsets=off)
+        for g in (1, 2, 4):
+            lo, hi = int(off[g]), int(off[g + 1])
+            ref = x[lo:hi].double() @ w4_values(w[g], s[g], run, w_fmt, None if z is None else z[g]).t().contiguous()
+            bound = (62.0 if w_fmt == 0 else 6.0) * scale_values(s[g]).repeat_interleave(run, -1)
+            assert ((y[lo:hi].double() - ref).abs() <= tolerance(x[lo:hi].double(), None, bound, torch.float32, ref)).all()
+
+
+def test_odd_places_of_scales(pkg):
+    """Scales and zero points that cannot be read 16 bytes at a time: off 16 bytes, rows that are not whole pieces."""
+    gen = generator("odd")
+    for k, run in ((1024, 32), (1152, 128), (1024, 128)):
+        n = 50
+        w, s, z = weights(gen, (), n, k, run, 0, torch.float16, True)
+        x = torch.randn((5, k), generator=gen, device="cuda").to(torch.bfloat16)
+        want = pkg.gemv_w4(x, w, s, run, zeros=z)
+        for shift in (1, 4):
+            s2 = torch.zeros(s.numel() + 8, dtype=s.dtype, device="cuda")[shift:shift + s.numel()].view(s.shape).copy_(s)
+            z2 = torch.zeros(z.numel() + 8, dtype=z.dtype, device="cuda")[shift:shift + z.numel()].view(z.shape).copy_(z)
+            assert torch.equal(pkg.gemv_w4(x, w, s2, run, zeros=z2), want)
+
+
 def test_captured_and_replayed_with_other_rows(pkg):
     gen = generator("graph")
     w, s, z = weights(gen, (4,), 256, 512, 64, 0, torch.float16, True)
