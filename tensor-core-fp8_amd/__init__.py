@@ -500,9 +500,13 @@ def _offsets(t):
     return _ints(t, "row_offsets"), t.shape[0] - 1
 
 
-def _output(out, shape, dtype, like):
+def _output(out, shape, dtype, like, stream):
+    """out, checked, or a new result: memory of the stream that writes it, so that nothing queued elsewhere still uses it."""
     if out is None:
-        return like.new_empty(shape, dtype=dtype or _torch.float32)
+        if stream is None:
+            return like.new_empty(shape, dtype=dtype or _torch.float32)
+        with _torch.cuda.stream(stream):
+            return like.new_empty(shape, dtype=dtype or _torch.float32)
     if out.shape != shape or not out.is_contiguous() or (dtype is not None and out.dtype != dtype):
         raise Fp8GemmError("out must be a contiguous %s tensor of the wanted type" % (shape,))
     return out
@@ -537,8 +541,8 @@ def quantize_rows(x, fmt=E4M3, row_index=None, codes=None, scales=None, stream=N
     L = _setup() if _torch is None else lib()
     rows, x_rows, cols, x_type, stride = _wide_matrix(x, row_index)
     device = _device_of(x, row_index, codes, scales)
-    codes = _output(codes, (rows, cols), _fp8_dtype(fmt), x)
-    scales = _output(scales, (rows,), _torch.float32, x)
+    codes = _output(codes, (rows, cols), _fp8_dtype(fmt), x, stream)
+    scales = _output(scales, (rows,), _torch.float32, x, stream)
     _launch(L.fp8gemm_quantize_rows, device, stream, rows, cols, x.data_ptr(), x_type, stride, x_rows,
             None if row_index is None else _ints(row_index, "row_index"), fmt, codes.data_ptr(), scales.data_ptr())
     return codes, scales
@@ -553,8 +557,8 @@ def quantize_columns(x, row_offsets, fmt=E4M3, row_index=None, codes=None, scale
     device = _device_of(x, row_offsets, row_index, codes, scales)
     offs, groups = _offsets(row_offsets)
     ld = grouped_ld(rows, groups)
-    codes = _output(codes, (cols, ld), _fp8_dtype(fmt), x)
-    scales = _output(scales, (groups, cols), _torch.float32, x)
+    codes = _output(codes, (cols, ld), _fp8_dtype(fmt), x, stream)
+    scales = _output(scales, (groups, cols), _torch.float32, x, stream)
     _launch(L.fp8gemm_quantize_columns, device, stream, groups, rows, cols, offs, x.data_ptr(), x_type, stride, x_rows,
             None if row_index is None else _ints(row_index, "row_index"), fmt, codes.data_ptr(), ld, scales.data_ptr())
     return codes, scales
@@ -575,7 +579,7 @@ def gemm_grouped(a, b, row_offsets, a_scale=None, b_scale=None, out_dtype=None, 
     if b.shape[0] != groups:
         raise Fp8GemmError("row_offsets is for %d experts, b holds %d" % (groups, b.shape[0]))
     (m, k), n = a.shape, b.shape[1]
-    out = _output(out, (m, n), out_dtype, a)
+    out = _output(out, (m, n), out_dtype, a, stream)
     per_column = b_scale is not None and b_scale.dim() == 2
     _launch(L.fp8gemm_grouped_tuned, device, stream, groups, m, k, n, offs, a.data_ptr(), _fp8_code(a, a_fmt), b.data_ptr(),
             _fp8_code(b, b_fmt), out.data_ptr(), _wide_code(out.dtype), _floats(a_scale, m, "a_scale"),
@@ -598,7 +602,7 @@ def gemm_grouped_wgrad(a_t, b_t, row_offsets, rows, a_scale=None, b_scale=None, 
         raise Fp8GemmError("accumulate needs the tensor to add to")
     offs, groups = _offsets(row_offsets)
     (m, ld), n = a_t.shape, b_t.shape[0]
-    out = _output(out, (groups, m, n), out_dtype, a_t)
+    out = _output(out, (groups, m, n), out_dtype, a_t, stream)
     _launch(L.fp8gemm_grouped_wgrad_tuned, device, stream, groups, rows, m, n, offs, a_t.data_ptr(), _fp8_code(a_t, a_fmt),
             b_t.data_ptr(), _fp8_code(b_t, b_fmt), ld, out.data_ptr(), _wide_code(out.dtype), _floats(a_scale, groups * m, "a_scale"),
             _floats(b_scale, groups * n, "b_scale"), int(bool(accumulate)), variant)
@@ -639,7 +643,7 @@ def gemv_w4(x, w, scales, run, w_fmt=W4_INT, zeros=None, x_scale=None, row_offse
         x_type = T_F16
     else:
         x_type = T_E4M3 if _fp8_code(x, x_fmt) == E4M3 else T_E5M2
-    out = _output(out, (m, n), out_dtype, x)
+    out = _output(out, (m, n), out_dtype, x, stream)
     args = (m, k, n, x.data_ptr(), x_type, _floats(x_scale, m, "x_scale"), w.data_ptr(), w_fmt, run, scales.data_ptr(), scale_type,
             None if zeros is None else zeros.data_ptr(), out.data_ptr(), _wide_code(out.dtype))
     if offs is None:
