@@ -512,8 +512,13 @@ def _output(out, shape, dtype, like, stream):
     return out
 
 
+def _fill(t, value, stream):
+    with _torch.cuda.stream(stream):
+        t.fill_(value)
+
+
 def grouped_ld(rows, groups):
-    """Columns of a transposed operand of gemm_grouped_wgrad for `rows` rows in `groups` experts."""
+    """Columns of a transposed operand of gemm_grouped_wgrad for `rows` rows in `groups` experts (0 for no rows)."""
     return lib().fp8gemm_grouped_ld(rows, groups)
 
 
@@ -543,6 +548,8 @@ def quantize_rows(x, fmt=E4M3, row_index=None, codes=None, scales=None, stream=N
     device = _device_of(x, row_index, codes, scales)
     codes = _output(codes, (rows, cols), _fp8_dtype(fmt), x, stream)
     scales = _output(scales, (rows,), _torch.float32, x, stream)
+    if rows == 0:
+        return codes, scales
     _launch(L.fp8gemm_quantize_rows, device, stream, rows, cols, x.data_ptr(), x_type, stride, x_rows,
             None if row_index is None else _ints(row_index, "row_index"), fmt, codes.data_ptr(), scales.data_ptr())
     return codes, scales
@@ -559,6 +566,9 @@ def quantize_columns(x, row_offsets, fmt=E4M3, row_index=None, codes=None, scale
     ld = grouped_ld(rows, groups)
     codes = _output(codes, (cols, ld), _fp8_dtype(fmt), x, stream)
     scales = _output(scales, (groups, cols), _torch.float32, x, stream)
+    if rows == 0:
+        _fill(scales, 1.0, stream)
+        return codes, scales
     _launch(L.fp8gemm_quantize_columns, device, stream, groups, rows, cols, offs, x.data_ptr(), x_type, stride, x_rows,
             None if row_index is None else _ints(row_index, "row_index"), fmt, codes.data_ptr(), ld, scales.data_ptr())
     return codes, scales
@@ -580,6 +590,8 @@ def gemm_grouped(a, b, row_offsets, a_scale=None, b_scale=None, out_dtype=None, 
         raise Fp8GemmError("row_offsets is for %d experts, b holds %d" % (groups, b.shape[0]))
     (m, k), n = a.shape, b.shape[1]
     out = _output(out, (m, n), out_dtype, a, stream)
+    if m == 0:
+        return out
     per_column = b_scale is not None and b_scale.dim() == 2
     _launch(L.fp8gemm_grouped_tuned, device, stream, groups, m, k, n, offs, a.data_ptr(), _fp8_code(a, a_fmt), b.data_ptr(),
             _fp8_code(b, b_fmt), out.data_ptr(), _wide_code(out.dtype), _floats(a_scale, m, "a_scale"),
@@ -603,6 +615,10 @@ def gemm_grouped_wgrad(a_t, b_t, row_offsets, rows, a_scale=None, b_scale=None, 
     offs, groups = _offsets(row_offsets)
     (m, ld), n = a_t.shape, b_t.shape[0]
     out = _output(out, (groups, m, n), out_dtype, a_t, stream)
+    if rows == 0:
+        if not accumulate:
+            _fill(out, 0.0, stream)
+        return out
     _launch(L.fp8gemm_grouped_wgrad_tuned, device, stream, groups, rows, m, n, offs, a_t.data_ptr(), _fp8_code(a_t, a_fmt),
             b_t.data_ptr(), _fp8_code(b_t, b_fmt), ld, out.data_ptr(), _wide_code(out.dtype), _floats(a_scale, groups * m, "a_scale"),
             _floats(b_scale, groups * n, "b_scale"), int(bool(accumulate)), variant)
@@ -644,6 +660,8 @@ def gemv_w4(x, w, scales, run, w_fmt=W4_INT, zeros=None, x_scale=None, row_offse
     else:
         x_type = T_E4M3 if _fp8_code(x, x_fmt) == E4M3 else T_E5M2
     out = _output(out, (m, n), out_dtype, x, stream)
+    if m == 0:
+        return out
     args = (m, k, n, x.data_ptr(), x_type, _floats(x_scale, m, "x_scale"), w.data_ptr(), w_fmt, run, scales.data_ptr(), scale_type,
             None if zeros is None else zeros.data_ptr(), out.data_ptr(), _wide_code(out.dtype))
     if offs is None:

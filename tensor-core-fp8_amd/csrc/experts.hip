@@ -95,6 +95,8 @@ namespace {
 
 static_assert(kMaxGroups == FP8GEMM_MAX_GROUPS, "the header names the table's size");
 
+// a number of rows, columns or k: with room for the rounding up that grids and kernels do in ints
+bool size_ok(int n) { return n > 0 && n <= (1 << 30); }
 bool fmt_ok(int f) { return f == FP8GEMM_E4M3 || f == FP8GEMM_E5M2; }
 bool wide_ok(int t) { return t == FP8GEMM_OUT_F32 || t == FP8GEMM_OUT_BF16 || t == FP8GEMM_OUT_F16; }
 bool aligned_to(const void *p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -104,7 +106,7 @@ bool wide_aligned(const void *p, int type) { return aligned_to(p, type == FP8GEM
 int grouped(int groups, int m, int k, int n, const int *row_offsets, const void *a, int a_fmt, const void *b, int b_fmt, void *out, int out_type,
             const float *a_scale, const float *b_scale, int b_scale_per_column, int variant, void *stream)
 {
-    if (groups <= 0 || groups > kMaxGroups || m <= 0 || k <= 0 || n <= 0 || !row_offsets || !a || !b || !out) return (int)hipErrorInvalidValue;
+    if (groups <= 0 || groups > kMaxGroups || !size_ok(m) || !size_ok(k) || !size_ok(n) || !row_offsets || !a || !b || !out) return (int)hipErrorInvalidValue;
     if (!fmt_ok(a_fmt) || !fmt_ok(b_fmt) || !wide_ok(out_type) || !wide_aligned(out, out_type)) return (int)hipErrorInvalidValue;
     const uint8_t *pa = static_cast<const uint8_t *>(a), *pb = static_cast<const uint8_t *>(b);
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -119,7 +121,7 @@ int grouped(int groups, int m, int k, int n, const int *row_offsets, const void 
 int wgrad(int groups, int rows, int m, int n, const int *row_offsets, const void *a_t, int a_fmt, const void *b_t, int b_fmt, int ld, void *out,
           int out_type, const float *a_scale, const float *b_scale, int accumulate, int variant, void *stream)
 {
-    if (groups <= 0 || groups > kMaxGroups || rows <= 0 || m <= 0 || n <= 0 || !row_offsets || !a_t || !b_t || !out) return (int)hipErrorInvalidValue;
+    if (groups <= 0 || groups > kMaxGroups || rows <= 0 || !size_ok(m) || !size_ok(n) || !row_offsets || !a_t || !b_t || !out) return (int)hipErrorInvalidValue;
     if (!fmt_ok(a_fmt) || !fmt_ok(b_fmt) || !wide_ok(out_type) || !wide_aligned(out, out_type)) return (int)hipErrorInvalidValue;
     const int least = fp8gemm_grouped_ld(rows, groups);
     if (least == 0 || ld < least || ld % kTokenRun != 0 || ld > (1 << 23)) return (int)hipErrorInvalidValue;
@@ -135,27 +137,42 @@ int wgrad(int groups, int rows, int m, int n, const int *row_offsets, const void
 }
 
 // ------------------------------------------------------------------ quantisation
+constexpr int kRowsAtOnce = 1 << 23;                       // rows of one launch: 2^32 threads are too many for a grid
+
 template <int TYPE, int FMT>
 hipError_t launch_quantize_rows(int rows, int cols, const void *x, size_t stride, int x_rows, const int *index, uint8_t *codes, float *scales, hipStream_t s)
 {
     const size_t elem = TYPE == FP8GEMM_OUT_F32 ? 4 : 2;
     const bool vec = cols % 8 == 0 && aligned_to(x, 16) && stride * elem % 16 == 0 && aligned_to(codes, 8);
-#define ROWS_KERNEL(WAVES, HELD)                                                                                                              \
-    hipLaunchKernelGGL((quantize_rows_kernel<TYPE, FMT, WAVES, HELD>), dim3((unsigned)((rows + 4 / WAVES - 1) / (4 / WAVES))), dim3(256), 0, s, \
-                       rows, cols, x, stride, x_rows, index, codes, scales)
-    // Four waves to a row, two or eight pieces of eight elements a lane; short rows get a wave each, for which four would be
-    // half idle.  One wave with eight pieces for rows of 4096 is slower: 32768 rows 109 us against 97, 3001 rows of
-    // 2048 11.6 against 9.8 (other data read in between, so that x is not cached).
-    if (vec && cols <= 1024)
-        ROWS_KERNEL(1, 2);
-    else if (vec && cols <= 4096)
-        ROWS_KERNEL(4, 2);
-    else if (vec && cols <= 16384)
-        ROWS_KERNEL(4, 8);
-    else
-        hipLaunchKernelGGL((quantize_rows_any_kernel<TYPE, FMT>), dim3((unsigned)rows), dim3(256), 0, s, cols, x, stride, x_rows, index, codes, scales);
+    for (; rows > 0; rows -= kRowsAtOnce) {
+        const int now = std::min(rows, kRowsAtOnce);
+#define ROWS_KERNEL(WAVES, HELD)                                                                                                            \
+    hipLaunchKernelGGL((quantize_rows_kernel<TYPE, FMT, WAVES, HELD>), dim3((unsigned)((now + 4 / WAVES - 1) / (4 / WAVES))), dim3(256), 0, s, \
+                       now, cols, x, stride, x_rows, index, codes, scales)
+        // Four waves to a row, two or eight pieces of eight elements a lane; short rows get a wave each, for which four would be
+        // half idle.  One wave with eight pieces for rows of 4096 is slower: 32768 rows 109 us against 97, 3001 rows of
+        // 2048 11.6 against 9.8 (other data read in between, so that x is not cached).
+        if (vec && cols <= 1024)
+            ROWS_KERNEL(1, 2);
+        else if (vec && cols <= 4096)
+            ROWS_KERNEL(4, 2);
+        else if (vec && cols <= 16384)
+            ROWS_KERNEL(4, 8);
+        else
+            hipLaunchKernelGGL((quantize_rows_any_kernel<TYPE, FMT>), dim3((unsigned)now), dim3(256), 0, s, cols, x, stride, x_rows, index, codes, scales);
 #undef ROWS_KERNEL
-    return hipGetLastError();
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        if (index)
+            index += now;
+        else {
+            x = static_cast<const char *>(x) + (size_t)now * stride * elem;
+            x_rows -= now;
+        }
+        codes += (size_t)now * cols;
+        scales += now;
+    }
+    return hipSuccess;
 }
 
 template <int TYPE, int FMT>
@@ -166,7 +183,7 @@ hipError_t launch_quantize_columns(const GroupSpec &grp, int cols, const void *x
     const bool vec = cols % 8 == 0 && aligned_to(x, 16) && stride * elem % 16 == 0;
     const long col_blocks = (cols + kColBlock - 1) / kColBlock;
     const long grid = col_blocks * (grp.groups + 1);
-    if (grid > 0x7FFFFFFFL) return hipErrorInvalidValue;
+    if (grid > 0xFFFFFFFFL / kColThreads) return hipErrorInvalidValue;
     if (vec)
         hipLaunchKernelGGL((quantize_columns_kernel<TYPE, FMT, true>), dim3((unsigned)grid), dim3(kColThreads), 0, s, grp, cols, x, stride, x_rows, index, codes, ld,
                            scales);
@@ -178,7 +195,7 @@ hipError_t launch_quantize_columns(const GroupSpec &grp, int cols, const void *x
 
 bool quantize_source_ok(int rows, int cols, const void *x, int x_type, long long x_stride, int x_rows, const int *row_index, int fmt)
 {
-    if (rows <= 0 || cols <= 0 || x_rows <= 0 || !x || !wide_ok(x_type) || !fmt_ok(fmt) || x_stride < cols) return false;
+    if (!size_ok(rows) || !size_ok(cols) || x_rows <= 0 || !x || !wide_ok(x_type) || !fmt_ok(fmt) || x_stride < cols) return false;
     return (row_index || rows <= x_rows) && wide_aligned(x, x_type);
 }
 
@@ -186,7 +203,7 @@ bool quantize_source_ok(int rows, int cols, const void *x, int x_type, long long
 int gemv_w4(int groups, int m, int k, int n, const int *row_offsets, const void *x, int x_type, const float *x_scale, const void *w, int w_fmt, int run,
             const void *w_scales, int scale_type, const void *w_zeros, void *y, int y_type, void *stream)
 {
-    if (groups <= 0 || groups > kMaxGroups || m <= 0 || k <= 0 || n <= 0 || run <= 0 || !x || !w || !w_scales || !y) return (int)hipErrorInvalidValue;
+    if (groups <= 0 || groups > kMaxGroups || !size_ok(m) || !size_ok(k) || !size_ok(n) || run <= 0 || !x || !w || !w_scales || !y) return (int)hipErrorInvalidValue;
     if (run % 32 != 0 || k % run != 0 || k > (1 << 23)) return (int)hipErrorInvalidValue;
     if (w_fmt != FP8GEMM_W4_INT && w_fmt != FP8GEMM_W4_E2M1) return (int)hipErrorInvalidValue;
     if (w_zeros && w_fmt != FP8GEMM_W4_INT) return (int)hipErrorInvalidValue;

@@ -22,14 +22,14 @@ static hipError_t launch_grouped_shape(int m, int k, int n, const uint8_t *a, co
     constexpr int kFixedLds = S::PTILE_LDS_BYTES + kGroupTableOffset + 2 * (S::BM + S::BN) * 4;
     static_assert(kFixedLds + kGroupTableBytes <= S::LDS_MAX, "the group table does not fit behind the ring");
     static_assert((kFixedLds + 2 * 257 * 4) * PER_CU <= S::LDS_MAX, "two workgroups of up to 256 groups do not fit a CU");
-    const int lds = kFixedLds + 2 * (grp.groups + 1) * 4;
-    auto kernel = gemm_ptile_grouped_kernel<S, AF, BF, KOVER, BSTREAM, NOPF, GROUPED, PER_CU>;
-    hipError_t e = allow_lds<PtileGroupedKernelTag<S, AF, BF, KOVER, BSTREAM, NOPF, GROUPED, PER_CU>>(kernel, kFixedLds + kGroupTableBytes);
-    if (e != hipSuccess) return e;
     const int tiles_m = (m + S::BM - 1) / S::BM, tiles_n = (n + S::BN - 1) / S::BN;
     // tile numbers are ints (the rows of every group may leave a tile of their own)
     const long tiles = GROUPED == kGroupedRows ? ((long)tiles_m + grp.groups) * tiles_n : (long)tiles_m * tiles_n * grp.groups;
     if (tiles > (1L << 30)) return hipErrorInvalidValue;
+    const int lds = kFixedLds + 2 * (grp.groups + 1) * 4;
+    auto kernel = gemm_ptile_grouped_kernel<S, AF, BF, KOVER, BSTREAM, NOPF, GROUPED, PER_CU>;
+    hipError_t e = allow_lds<PtileGroupedKernelTag<S, AF, BF, KOVER, BSTREAM, NOPF, GROUPED, PER_CU>>(kernel, kFixedLds + kGroupTableBytes);
+    if (e != hipSuccess) return e;
     const unsigned grid = tiles < 256 * PER_CU ? (unsigned)((tiles + 7) / 8 * 8) : 256u * PER_CU;
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(S::THREADS), lds, stream, m, k, n, a, b, out, tiles_m, tiles_n, rotate, grp);
     return hipGetLastError();
@@ -55,7 +55,7 @@ hipError_t dispatch_grouped(int m, int k, int n, const uint8_t *a, const uint8_t
     switch (variant) {
     case kGroupedDirect: {
         const long tiles_m = (m + 31) / 32, tiles_n = (n + 31) / 32;
-        if (tiles_m * tiles_n > 0x7FFFFFFFL) return hipErrorInvalidValue;
+        if (tiles_m * tiles_n > 0xFFFFFFFFL / 64) return hipErrorInvalidValue;          // (a grid holds fewer than 2^32 threads)
         hipLaunchKernelGGL((gemm_grouped_direct_kernel<AF, BF>), dim3((unsigned)(tiles_m * tiles_n)), dim3(64), 0, stream, k, n, a, b, out, (int)tiles_n,
                            aligned ? 1 : 0, grp);
         return hipGetLastError();

@@ -53,6 +53,17 @@ def test_quantize(pkg):
     refused(pkg.lib().fp8gemm_quantize_columns, QCOLS, common + [dict(codes_t=None), dict(codes_t=ODD), dict(row_offsets=None), dict(groups=0), dict(groups=2000), dict(ld=256), dict(ld=500), dict(rows=1 << 24, x_rows=1 << 24)])
 
 
+def test_sizes_beyond_the_grids(pkg):
+    """More than 2^30 of anything, or more workgroups than a grid holds."""
+    big = (1 << 30) + 1
+    refused(pkg.lib().fp8gemm_grouped, GROUPED, [dict(m=big), dict(k=big), dict(n=big), dict(m=2 ** 31 - 1), dict(m=1 << 30, n=1 << 30)])
+    refused(pkg.lib().fp8gemm_grouped, dict(GROUPED, a=ODD), [dict(m=1 << 21, n=1 << 21), dict(m=1 << 30, n=1 << 30)])
+    refused(pkg.lib().fp8gemm_grouped_wgrad, WGRAD, [dict(m=big), dict(n=big), dict(m=2 ** 31 - 1), dict(m=1 << 30, n=1 << 30), dict(rows=2 ** 31 - 1)])
+    refused(pkg.lib().fp8gemm_quantize_rows, QROWS, [dict(rows=big, x_rows=2 ** 31 - 1), dict(cols=big, x_stride=big)])
+    refused(pkg.lib().fp8gemm_quantize_columns, dict(QCOLS, groups=1024, ld=131200), [dict(cols=1 << 24, x_stride=1 << 24), dict(cols=2 ** 31 - 1, x_stride=1 << 40)])
+    refused(pkg.lib().fp8gemm_gemv_w4, W4, [dict(m=big), dict(n=big), dict(n=2 ** 31 - 1), dict(m=2 ** 31 - 1)])
+
+
 def test_padded_length(pkg):
     """Whole runs of 128 for every expert, whatever the cut; 0 for what is no length."""
     ld = pkg.lib().fp8gemm_grouped_ld

@@ -154,3 +154,38 @@ def test_operands_on_another_stream_and_wrong_places(pkg):
                 lambda: pkg.gemv_w4(a.to(torch.bfloat16), b.view(torch.uint8)[0, :, :64].contiguous(), torch.ones(64, 3, device="cuda"), 32)):
         with pytest.raises((pkg.Fp8GemmError, TypeError)):
             bad()
+
+
+def test_a_step_without_tokens(pkg):
+    """No token came: empty products, gradients of zeros, or nothing added."""
+    off = torch.zeros(4, dtype=torch.int32, device="cuda")
+    x, g = (torch.zeros((0, c), dtype=torch.bfloat16, device="cuda") for c in (64, 32))
+    w = codes(generator("no tokens"), (3, 32, 64), 0)
+    xc, xs = pkg.quantize_rows(x)
+    assert pkg.gemm_grouped(xc, w, off, a_scale=xs, out_dtype=torch.bfloat16).shape == (0, 32)
+    xt, xts = pkg.quantize_columns(x, off)
+    gt, gts = pkg.quantize_columns(g, off)
+    dw = pkg.gemm_grouped_wgrad(gt, xt, off, 0, a_scale=gts, b_scale=xts)
+    assert dw.shape == (3, 32, 64) and not dw.any()
+    held = torch.full((3, 32, 64), 2.0, device="cuda")
+    pkg.gemm_grouped_wgrad(gt, xt, off, 0, out=held, accumulate=True)
+    assert (held == 2.0).all()
+    w4 = torch.zeros((3, 32, 32), dtype=torch.uint8, device="cuda")
+    assert pkg.gemv_w4(x, w4, torch.ones((3, 32, 2), device="cuda"), 32, row_offsets=off).shape == (0, 32)
+
+
+def test_results_on_a_named_stream_are_its_memory(pkg):
+    """Work still queued on the current stream does not reach memory that another stream's call was given."""
+    gen = generator("named")
+    x = torch.randn((4096, 4096), generator=gen, device="cuda").to(torch.bfloat16)
+    want, want_s = pkg.quantize_rows(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        late = torch.empty((4096, 4096), dtype=torch.uint8, device="cuda")
+        for _ in range(8):
+            late.fill_(0x55)
+        del late                                                # (its writes may still be queued)
+        got, got_s = pkg.quantize_rows(x, stream=side)
+        torch.cuda.synchronize()
+        assert torch.equal(got.view(torch.uint8), want.view(torch.uint8)) and torch.equal(got_s, want_s)

@@ -170,6 +170,31 @@ def test_smallest_numbers(pkg):
     same(got, v)
 
 
+@pytest.mark.parametrize("rows,cols,gathered", [((1 << 26) + 5, 8, False), ((1 << 24) + 3, 3, False), ((1 << 24) + 3, 3, True), ((1 << 23) + 1, 1032, True)])
+def test_more_rows_than_a_grid_holds(pkg, rows, cols, gathered):
+    gen = generator("rows %d" % rows)
+    x = torch.randn((1000 if gathered else rows, cols), generator=gen, device="cuda", dtype=torch.bfloat16)
+    index = torch.arange(rows, device="cuda", dtype=torch.int32).remainder_(1001) if gathered else None      # (1000: a row of zeros)
+    got, scales = pkg.quantize_rows(x, 0, row_index=index)
+    for lo in (0, (1 << 23) - 4, rows - 9):
+        at = slice(lo, lo + 9)
+        part = x[at] if index is None else torch.cat([x, torch.zeros_like(x[:1])])[index[at].long()]
+        v, s = quantized(part, 0, 1)
+        lo_end = min(rows, lo + 9)
+        assert torch.equal(scales[lo:lo_end].double(), s)
+        same(got[lo:lo_end], v)
+
+
+def test_no_rows(pkg):
+    x = torch.zeros((0, 72), device="cuda")
+    codes, scales = pkg.quantize_rows(x)
+    assert codes.shape == (0, 72) and scales.shape == (0,)
+    codes, scales = pkg.quantize_rows(torch.ones((5, 72), device="cuda"), row_index=torch.zeros(0, dtype=torch.int32, device="cuda"))
+    assert codes.shape == (0, 72) and scales.shape == (0,)
+    codes, scales = pkg.quantize_columns(x, torch.zeros(4, dtype=torch.int32, device="cuda"))
+    assert codes.shape == (72, 0) and torch.equal(scales, torch.ones((3, 72), device="cuda"))
+
+
 def test_columns_of_many_experts(pkg):
     gen = generator("1024")
     counts = [0] * 1024
