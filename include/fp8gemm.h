@@ -190,7 +190,7 @@ int fp8gemm_quantize_rows(int rows, int cols, const void *x, int x_type, long lo
 int fp8gemm_quantize_columns(int groups, int rows, int cols, const int *row_offsets, const void *x, int x_type, long long x_stride,
                              int x_rows, const int *row_index, int fmt, void *codes_t, int ld, float *scales, void *stream);
 /*
- * Matrix-vector products with 4-bit weights, for few rows of x (the weights are read once per 64 rows):
+ * Matrix-vector products with 4-bit weights, for few rows of x (the weights are read once per 16 to 64 rows):
  *     y[i * n + j] = cast( x_scale[i] * sum_{t<k} x[i * k + t] * value(i, j, t) ),
  *     value = (nibble - zero) * scale  (FP8GEMM_W4_INT) or e2m1(nibble) * scale (FP8GEMM_W4_E2M1: sign, two bits
  *     of exponent, one of mantissa: 0 0.5 1 1.5 2 3 4 6)

@@ -21,6 +21,7 @@
 // A workgroup of eight waves is WC waves side by side (16 columns each) times WK waves along K, whose sums are
 // added in wave order through LDS: few columns still fill the chip.  It goes through several blocks of columns;
 // x and the scales of all of them are staged in LDS once, then the waves' rings run without a break over all blocks.
+// One row, 28672 x 8192 integers in runs of 128: 27 us, 4.5 TB/s; runs of 32 43 us, where the vector unit is the bound.
 #ifndef FP8GEMM_KERNEL_W4_H
 #define FP8GEMM_KERNEL_W4_H
 
@@ -80,27 +81,17 @@ __device__ __forceinline__ v4f w4_mfma(v4i a, v4i b, v4f c)
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
-// eight consecutive numbers of x as 16-bit ones (f16 from fp8 codes: exact)
-template <bool F16>
-__device__ __forceinline__ v4i w4_load_x(const void *x, size_t index, int type)
+// eight codes of x as f16 numbers (exact); both formats are expanded and one picked, so that the callers' loops stay without branches
+__device__ __forceinline__ v4i w4_widen(v2u c, int type)
 {
-    if (!F16 || type == FP8GEMM_T_F16) return *reinterpret_cast<const v4i *>(static_cast<const unsigned short *>(x) + index);
-    const v2u c = *reinterpret_cast<const v2u *>(static_cast<const uint8_t *>(x) + index);
     v4i r;
-    if (type == FP8GEMM_T_E5M2) {                       // the upper byte of an f16
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            r[2 * h] = (int)(((c[h] & 0xFFu) << 8) | ((c[h] & 0xFF00u) << 16));
-            r[2 * h + 1] = (int)(((c[h] >> 8) & 0xFF00u) | (c[h] & 0xFF000000u));
-        }
-    } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[h], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[h], true);
-            const _Float16 f[4] = {(_Float16)lo[0], (_Float16)lo[1], (_Float16)hi[0], (_Float16)hi[1]};
-            r[2 * h] = (int)((uint32_t)__builtin_bit_cast(unsigned short, f[0]) | ((uint32_t)__builtin_bit_cast(unsigned short, f[1]) << 16));
-            r[2 * h + 1] = (int)((uint32_t)__builtin_bit_cast(unsigned short, f[2]) | ((uint32_t)__builtin_bit_cast(unsigned short, f[3]) << 16));
-        }
+    for (int h = 0; h < 2; ++h) {
+        const int lo = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[h], 1.0f, false));
+        const int hi = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c[h], 1.0f, true));
+        // (e5m2: the upper byte of an f16)
+        r[2 * h] = type == FP8GEMM_T_E5M2 ? (int)__builtin_amdgcn_perm(0u, c[h], 0x010C000Cu) : lo;
+        r[2 * h + 1] = type == FP8GEMM_T_E5M2 ? (int)__builtin_amdgcn_perm(0u, c[h], 0x030C020Cu) : hi;
     }
     return r;
 }
@@ -116,6 +107,57 @@ __host__ __device__ constexpr int w4_x_pitch(int chunk) { return chunk * 2 + 16;
 __host__ __device__ constexpr int w4_scale_pitch(int runs, int entry) { return ((runs * entry + 15) / 16 | 1) * 16; }
 // two sets of the partial sums of the waves along K: rows x 16 floats a wave
 __host__ __device__ constexpr int w4_part_bytes(int wk, int rows) { return wk > 1 ? 2 * (wk - 1) * (kW4Waves / wk) * rows * 64 : 0; }
+
+// eight numbers of x as the weights are expanded: integers 0 4, 1 5, 2 6, 3 7
+template <int MODE>
+__device__ __forceinline__ v4i w4_order(v4i t)
+{
+    if (MODE != kW4Int) return t;
+    return v4i{(int)__builtin_amdgcn_perm((uint32_t)t[2], (uint32_t)t[0], 0x05040100u), (int)__builtin_amdgcn_perm((uint32_t)t[2], (uint32_t)t[0], 0x07060302u),
+               (int)__builtin_amdgcn_perm((uint32_t)t[3], (uint32_t)t[1], 0x05040100u), (int)__builtin_amdgcn_perm((uint32_t)t[3], (uint32_t)t[1], 0x07060302u)};
+}
+
+// Stages `units` pieces of eight numbers of each of `rows` rows of x, row m0 on, from k = c0 on (zeros behind the last k), by the
+// first `threads` threads: piece after piece, row after row, kW4XLoads loads of a thread in flight.  CODES: x in fp8.
+constexpr int kW4XLoads = 4;
+template <int MODE, bool CODES>
+__device__ __forceinline__ void w4_stage_x(const W4Args &p, int m0, int rows, int c0, int units, LDS_AS uint8_t *xs, int x_pitch, int threads)
+{
+    int row = 0, u = threadIdx.x;
+    while (u >= units) {
+        u -= units;
+        ++row;
+    }
+    while (row < rows) {
+        v4i v[kW4XLoads];
+        int at[kW4XLoads];
+        bool there[kW4XLoads];
+#pragma unroll
+        for (int b = 0; b < kW4XLoads; ++b) {
+            at[b] = row < rows ? row * x_pitch + u * 16 : -1;
+            there[b] = row < rows && c0 + u * 8 < p.k;
+            // (a place outside reads the first numbers instead: no branch holds up the loads behind it)
+            const size_t from = there[b] ? (size_t)(m0 + row) * p.k + c0 + u * 8 : 0;
+            if (CODES) {
+                const v2u c = *reinterpret_cast<const v2u *>(static_cast<const uint8_t *>(p.x) + from);
+                v[b] = v4i{(int)c[0], (int)c[1], 0, 0};
+            } else {
+                v[b] = *reinterpret_cast<const v4i *>(static_cast<const unsigned short *>(p.x) + from);
+            }
+            u += threads;
+            while (u >= units) {
+                u -= units;
+                ++row;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < kW4XLoads; ++b) {
+            v4i o = w4_order<MODE>(CODES ? w4_widen(v2u{(uint32_t)v[b][0], (uint32_t)v[b][1]}, p.x_type) : v[b]);
+            if (!there[b]) o = v4i{0, 0, 0, 0};
+            if (at[b] >= 0) *reinterpret_cast<LDS_AS v4i *>(xs + at[b]) = o;
+        }
+    }
+}
 
 // -(16 + z) in 16 bits, twice: z in the top of the mantissa of -16
 template <bool F16>
@@ -250,11 +292,73 @@ __device__ __forceinline__ void w4_entry(const LDS_AS uint8_t *at, float &scale,
         scale = __builtin_bit_cast(float, bits << 23);
 }
 
+// the scales staged from the stored type, 16 bytes at a time where runs and addresses allow it
+template <bool F16, int MODE, int RUN, int KIND>
+__device__ __forceinline__ void w4_stage_scales_any(const W4Args &p, size_t at0, int first_k, int runs, int cols, int block_cols, LDS_AS uint8_t *out, int tid, int threads)
+{
+    const int es = p.scale_type == FP8GEMM_T_E8M0 ? 1 : (p.scale_type == FP8GEMM_T_F32 ? 4 : 2), last = 16 / es - 1;
+    const bool vec = p.run == RUN && ((p.per_row | runs | (first_k / RUN)) & last) == 0 && reinterpret_cast<uintptr_t>(p.w_scale) % 16 == 0 &&
+                     (!p.zeros || reinterpret_cast<uintptr_t>(p.zeros) % 16 == 0);
+#define W4_STAGE(ES) \
+    (vec ? w4_stage_scales<F16, MODE, RUN, KIND, ES, true>(p, at0, first_k, runs, cols, block_cols, out, tid, threads) \
+         : w4_stage_scales<F16, MODE, RUN, KIND, ES, false>(p, at0, first_k, runs, cols, block_cols, out, tid, threads))
+    if constexpr (KIND == kW4ScaleF32) {
+        W4_STAGE(4);
+    } else if constexpr (KIND == kW4ScaleByte) {
+        W4_STAGE(1);
+    } else {
+        if (KIND == kW4ScaleBf16 && es == 1)
+            W4_STAGE(1);
+        else
+            W4_STAGE(2);
+    }
+#undef W4_STAGE
+}
+
+// the rows of group g: offsets clamped to the matrix and raised to the largest before them (group_table.h)
+__device__ __forceinline__ void w4_group_rows(const W4Args &p, int g, int &first, int &end)
+{
+    first = 0;
+    end = p.rows;
+    if (!p.offsets) return;
+    GroupSpec spec = {};
+    spec.offsets = p.offsets;
+    spec.rows = p.rows;
+    int most = 0;
+    for (int i = threadIdx.x & 63; i <= g; i += 64) {
+        const int v = group_offset(spec, i);
+        most = v > most ? v : most;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const int v = __shfl_xor(most, off, 64);
+        most = v > most ? v : most;
+    }
+    first = __builtin_amdgcn_readfirstlane(most);
+    end = __builtin_amdgcn_readfirstlane(group_offset(spec, g + 1));
+}
+
+// an extent of `bytes` (2^32 - 16 at most) from `base` on
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t w4_rsrc(const void *base, size_t bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), 0, (int)(uint32_t)(bytes > 0xFFFFFFF0u ? 0xFFFFFFF0u : bytes), 0x00020000);
+}
+
+// Four lanes 16 apart hold 16 consecutive bytes each: afterwards word d of lane q is word q of lane d.
+__device__ __forceinline__ void w4_turn(uint32_t w[4])
+{
+    const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false), b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+    const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+    w[0] = c[0];
+    w[1] = c[1];
+    w[2] = d[0];
+    w[3] = d[1];
+}
+
 // F16: x and the expanded weights are f16 (else bf16).  RUN: 128 or 32, the k between two scales of the staged table.
-// MT: blocks of 16 rows of x held at once.
 // KIND: how the scales are staged.
-template <bool F16, int MODE, int RUN, int MT, int KIND>
-__global__ __launch_bounds__(64 * kW4Waves) void gemv_w4_kernel(W4Args p)
+template <bool F16, int MODE, int RUN, int KIND>
+__global__ __launch_bounds__(64 * kW4Waves, 4) void gemv_w4_kernel(W4Args p)
 {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const uint32_t lds_base = (uint32_t)(uintptr_t)(LDS_AS uint8_t *)lds;
@@ -268,26 +372,9 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemv_w4_kernel(W4Args p)
     const int block_n0 = blockIdx.x * block_cols * p.blocks;
     const int blocks = p.n - block_n0 < p.blocks * block_cols ? (p.n - block_n0 + block_cols - 1) >> (4 + kW4WavesShift - p.wk_shift) : p.blocks;
     const int n0 = block_n0 + 16 * wc;
-    int first = 0, end = p.rows;
-    if (p.offsets) {
-        // the group's rows: offsets clamped to the matrix and raised to the largest before them (group_table.h)
-        GroupSpec spec = {};
-        spec.offsets = p.offsets;
-        spec.rows = p.rows;
-        int most = 0;
-        for (int i = lane; i <= g; i += 64) {
-            const int v = group_offset(spec, i);
-            most = v > most ? v : most;
-        }
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) {
-            const int v = __shfl_xor(most, off, 64);
-            most = v > most ? v : most;
-        }
-        first = __builtin_amdgcn_readfirstlane(most);
-        end = __builtin_amdgcn_readfirstlane(group_offset(spec, g + 1));
-        if (end <= first) return;
-    }
+    int first, end;
+    w4_group_rows(p, g, first, end);
+    if (end <= first) return;
     const int fi = lane & 15, fq = lane >> 4;
 
     // ---- ring of this wave: 16 rows of W, kW4RowBytes of each a stage, 16-byte pieces swizzled by row
@@ -313,8 +400,8 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemv_w4_kernel(W4Args p)
     const int whole = (p.k + unit - 1) & ~(unit - 1);
     int flushed = 0;                                      // tiles added up so far: which of the two sets of partial sums is next
 
-    for (int m0 = first; m0 < end; m0 += 16 * MT) {
-        const int rows = end - m0 < 16 * MT ? end - m0 : 16 * MT;
+    for (int m0 = first; m0 < end; m0 += 16) {
+        const int rows = end - m0 < 16 ? end - m0 : 16;
         // Staged at a time: all of K of x, and the scales of as many blocks of columns as fit beside it; where not even one
         // does, a block at a time with K in equal pieces, whole ring stages for every wave along K (the host leaves room
         // for one), whole multiples of 2048 if they are longer.
@@ -335,18 +422,12 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemv_w4_kernel(W4Args p)
         chunk = __builtin_amdgcn_readfirstlane(chunk);
         pass = __builtin_amdgcn_readfirstlane(pass);
         const int runs = chunk / RUN, x_pitch = w4_x_pitch(chunk), s_pitch = w4_scale_pitch(runs, EB);
-        int x_row[MT];                                    // this lane's place in the staged x (past the last row: that one again)
-        float x_scale[MT][4];
+        // this lane's place in the staged x (past the last row: that one again)
+        const int x_row = (fi < rows ? fi : rows - 1) * x_pitch + (PER_LANE ? 4 * fq : fq) * 16;
+        float x_scale[4];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            x_row[i] = (i * 16 + fi < rows ? i * 16 + fi : rows - 1) * x_pitch + (PER_LANE ? 4 * fq : fq) * 16;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = i * 16 + 4 * fq + r;
-                x_scale[i][r] = p.x_scale && row < rows ? p.x_scale[m0 + row] : 1.0f;
-            }
-        }
-        v4f total[MT];
+        for (int r = 0; r < 4; ++r) x_scale[r] = p.x_scale && 4 * fq + r < rows ? p.x_scale[m0 + 4 * fq + r] : 1.0f;
+        v4f total = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int b0 = 0; b0 < blocks; b0 += pass) {
             const int nb = blocks - b0 < pass ? blocks - b0 : pass;
             for (int c0 = 0; c0 < p.k; c0 += chunk) {
@@ -373,69 +454,25 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemv_w4_kernel(W4Args p)
 #pragma unroll
                 for (int t = 0; t < kW4RingFour; ++t)
                     if (t < p.ring && left > 0) issue(t);
-                // x by the lower half of the waves and the scales by the upper half at the same time (all of them where x stays)
+                // x and the scales: little of x by the lower half of the waves and the scales by the upper half at the same time, more by
+                // all of them
                 const bool with_x = b0 == 0 || chunk < whole;
                 const int half = 32 * kW4Waves;
-                if (with_x && threadIdx.x < half) {
-                    const int units = chunk / 8;          // eight numbers of a row
-                    constexpr int XB = 4;                 // loads a thread has in flight
-                    // (pieces of eight numbers, row after row; a thread's place moves on by `half` pieces)
-                    int row = 0, u = threadIdx.x;
-                    while (u >= units) {
-                        u -= units;
-                        ++row;
-                    }
-                    while (row < rows) {
-                        v4i v[XB];
-                        int at[XB];
-#pragma unroll
-                        for (int b = 0; b < XB; ++b) {
-                            v[b] = v4i{0, 0, 0, 0};
-                            at[b] = row < rows ? row * x_pitch + u * 16 : -1;
-                            if (row < rows && c0 + u * 8 < p.k) v[b] = w4_load_x<F16>(p.x, (size_t)(m0 + row) * p.k + c0 + u * 8, p.x_type);
-                            u += half;
-                            while (u >= units) {
-                                u -= units;
-                                ++row;
-                            }
-                        }
-#pragma unroll
-                        for (int b = 0; b < XB; ++b) {
-                            if (MODE == kW4Int) {
-                                // in the order of the expanded nibbles: 0 4, 1 5, 2 6, 3 7
-                                const v4i o = v[b];
-                                v[b][0] = (int)__builtin_amdgcn_perm((uint32_t)o[2], (uint32_t)o[0], 0x05040100u);
-                                v[b][1] = (int)__builtin_amdgcn_perm((uint32_t)o[2], (uint32_t)o[0], 0x07060302u);
-                                v[b][2] = (int)__builtin_amdgcn_perm((uint32_t)o[3], (uint32_t)o[1], 0x05040100u);
-                                v[b][3] = (int)__builtin_amdgcn_perm((uint32_t)o[3], (uint32_t)o[1], 0x07060302u);
-                            }
-                            if (at[b] >= 0) *reinterpret_cast<LDS_AS v4i *>(xs + at[b]) = v[b];
-                        }
-                    }
+                const bool apart = rows * (chunk / 8) <= 2 * half * kW4XLoads;      // (two rounds of loads at most)
+                const int x_threads = apart ? half : 2 * half;
+                if (with_x && threadIdx.x < x_threads) {
+                    if (F16 && p.x_type != FP8GEMM_T_F16)
+                        w4_stage_x<MODE, true>(p, m0, rows, c0, chunk / 8, xs, x_pitch, x_threads);
+                    else
+                        w4_stage_x<MODE, false>(p, m0, rows, c0, chunk / 8, xs, x_pitch, x_threads);
                 }
                 LDS_AS uint8_t *ss = xs + rows * x_pitch;
-                if (!with_x || threadIdx.x >= half) {
+                if (!with_x || !apart || threadIdx.x >= half) {
                     const int col0 = block_n0 + b0 * block_cols, staged = nb * block_cols;
                     const int cols = p.n - col0 < staged ? p.n - col0 : staged;
                     const size_t at0 = ((size_t)g * p.n + col0) * p.per_row;
-                    const int es = p.scale_type == FP8GEMM_T_E8M0 ? 1 : (p.scale_type == FP8GEMM_T_F32 ? 4 : 2), last = 16 / es - 1;
-                    const bool vec = p.run == RUN && ((p.per_row | runs | (c0 / RUN)) & last) == 0 &&
-                                     reinterpret_cast<uintptr_t>(p.w_scale) % 16 == 0 && (!p.zeros || reinterpret_cast<uintptr_t>(p.zeros) % 16 == 0);
-                    const int tid = with_x ? threadIdx.x - half : threadIdx.x, threads = with_x ? half : 2 * half;
-#define W4_STAGE(ES) \
-    (vec ? w4_stage_scales<F16, MODE, RUN, KIND, ES, true>(p, at0, c0, runs, cols, staged, ss, tid, threads) \
-         : w4_stage_scales<F16, MODE, RUN, KIND, ES, false>(p, at0, c0, runs, cols, staged, ss, tid, threads))
-                    if constexpr (KIND == kW4ScaleF32) {
-                        W4_STAGE(4);
-                    } else if constexpr (KIND == kW4ScaleByte) {
-                        W4_STAGE(1);
-                    } else {
-                        if (KIND == kW4ScaleBf16 && es == 1)
-                            W4_STAGE(1);
-                        else
-                            W4_STAGE(2);
-                    }
-#undef W4_STAGE
+                    const int tid = with_x && apart ? threadIdx.x - half : threadIdx.x, threads = with_x && apart ? half : 2 * half;
+                    w4_stage_scales_any<F16, MODE, RUN, KIND>(p, at0, c0, runs, cols, staged, ss, tid, threads);
                 }
                 // (every load has landed: said here, so that the compiler does not wait for all of them inside the loop)
                 wait_vmcnt<0>();
@@ -463,9 +500,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemv_w4_kernel(W4Args p)
                 if (todo > 0) read_stage(0, now);
                 wait_lgkmcnt0();
                 for (int b = 0; b < nb; ++b) {
-                    if (c0 == 0)
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) total[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (c0 == 0) total = v4f{0.0f, 0.0f, 0.0f, 0.0f};
                     const LDS_AS uint8_t *s_block = ss + (b * block_cols + 16 * wc + fi) * s_pitch + (MODE == kW4Fp4Scaled && RUN == 32 ? fq : 0) * EB;
                     for (int t0 = 0; t0 < T; ++t0) {
                         if (left > 0) {
@@ -486,7 +521,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemv_w4_kernel(W4Args p)
 #pragma unroll
                         for (int h = 0; h < kW4StageK / 128; ++h) {
                             const uint32_t *w = now + 4 * h;
-                            v4f sum[MT], excess[MT];
+                            v4f sum, excess;
                             float lane_scale = 1.0f, s = 0.0f;
                             uint32_t pair = 0;
                             v4i minus;
@@ -500,22 +535,17 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemv_w4_kernel(W4Args p)
                                         w4_entry<MODE, KIND>(s_at + (h * RUNS128 + (RUN == 32 ? d : 0)) * EB, s, pair);
                                         minus = v4i{(int)pair, (int)pair, (int)pair, (int)pair};
                                     }
-#pragma unroll
-                                for (int i = 0; i < MT; ++i) {
-                                    const v4i a = *reinterpret_cast<const LDS_AS v4i *>(x_at + x_row[i] + h * 256 + (PER_LANE ? d : 4 * d) * 16);
-                                    if constexpr (MODE == kW4Fp4Scaled) {
-                                        total[i] = w4_mfma<F16>(a, wide, total[i]);
-                                    } else {
-                                        // (the excess in a chain of its own: the two do not wait for each other)
-                                        sum[i] = w4_mfma<F16>(a, wide, open ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : sum[i]);
-                                        if constexpr (MODE == kW4Int) excess[i] = w4_mfma<F16>(a, minus, open ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : excess[i]);
-                                    }
+                                const v4i a = *reinterpret_cast<const LDS_AS v4i *>(x_at + x_row + h * 256 + (PER_LANE ? d : 4 * d) * 16);
+                                if constexpr (MODE == kW4Fp4Scaled) {
+                                    total = w4_mfma<F16>(a, wide, total);
+                                } else {
+                                    // (the excess in a chain of its own: the two do not wait for each other)
+                                    sum = w4_mfma<F16>(a, wide, open ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : sum);
+                                    if constexpr (MODE == kW4Int) excess = w4_mfma<F16>(a, minus, open ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : excess);
                                 }
                                 if (MODE != kW4Fp4Scaled && (RUN == 32 || d == 3)) {
 #pragma unroll
-                                    for (int i = 0; i < MT; ++i)
-#pragma unroll
-                                        for (int r = 0; r < 4; ++r) total[i][r] += s * (MODE == kW4Int ? sum[i][r] + excess[i][r] : sum[i][r]);
+                                    for (int r = 0; r < 4; ++r) total[r] += s * (MODE == kW4Int ? sum[r] + excess[r] : sum[r]);
                                 }
                             }
                         }
@@ -528,18 +558,14 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemv_w4_kernel(W4Args p)
                     }
                     if (c0 + chunk < p.k) continue;
                     // ---- the waves along K, added in wave order (two sets of partial sums in turn: one barrier a tile);
-                    // register r of lane (fi, fq) holds y[16 i + 4 fq + r][column fi]
+                    // register r of lane (fi, fq) holds y[4 fq + r][column fi]
                     if (wk_count > 1) {
                         LDS_AS float *set = parts + (flushed & 1) * ((wk_count - 1) * wc_count * p.part_rows * 16);
                         ++flushed;
                         if (wk > 0)
 #pragma unroll
-                            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) {
-                                    const int row = i * 16 + 4 * fq + r;
-                                    if (row < rows) set[(((wk - 1) * wc_count + wc) * p.part_rows + row) * 16 + fi] = total[i][r];
-                                }
+                            for (int r = 0; r < 4; ++r)
+                                if (4 * fq + r < rows) set[(((wk - 1) * wc_count + wc) * p.part_rows + 4 * fq + r) * 16 + fi] = total[r];
                         wait_lgkmcnt0();
                         asm volatile("" ::: "memory");
                         __builtin_amdgcn_s_barrier();     // (the loads in flight go on)
@@ -547,25 +573,207 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemv_w4_kernel(W4Args p)
                         if (wk == 0)
                             for (int o = 1; o < wk_count; ++o)
 #pragma unroll
-                                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                                    for (int r = 0; r < 4; ++r) {
-                                        const int row = i * 16 + 4 * fq + r;
-                                        if (row < rows) total[i][r] += set[(((o - 1) * wc_count + wc) * p.part_rows + row) * 16 + fi];
-                                    }
+                                for (int r = 0; r < 4; ++r)
+                                    if (4 * fq + r < rows) total[r] += set[(((o - 1) * wc_count + wc) * p.part_rows + 4 * fq + r) * 16 + fi];
                     }
                     const int col = n0 + (b0 + b) * block_cols + fi;
                     if (wk == 0 && col < p.n) {
 #pragma unroll
-                        for (int i = 0; i < MT; ++i)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) {
-                                const int row = i * 16 + 4 * fq + r;
-                                if (row < rows) store_out(p.y, (size_t)(m0 + row) * p.n + col, total[i][r] * x_scale[i][r], p.y_type);
-                            }
+                        for (int r = 0; r < 4; ++r)
+                            if (4 * fq + r < rows) store_out(p.y, (size_t)(m0 + 4 * fq + r) * p.n + col, total[r] * x_scale[r], p.y_type);
                     }
                 }
             }
+        }
+    }
+}
+
+// The same for more rows of x than one block of 16 (16 * MT at a time), where x no longer fits LDS and the waves would wait for
+// it: K goes by in pieces of kW4PieceK, x through two LDS buffers and two sets of registers (a piece is read three pieces ahead), the
+// weights straight into registers four pieces ahead, the scales staged for as many pieces as fit.  A wave takes TN blocks of
+// 16 columns, so that a read of x from LDS feeds TN products: with one the LDS is what bounds 64 rows.  Two waves along K.
+//
+// Where the four lanes of a row have to share 32 consecutive weights (see above) their 16-byte loads are turned around by
+// swaps between lanes.  64 rows, integers in runs of 128: 4096 x 4096 21.5 us (the kernel above, in blocks of 64 rows, 69),
+// 17536 x 6784 with 58 rows 55 (100): the matrix unit, LDS and the vector unit take 0.4 to 0.8 us of a piece's 1.7 each, and two
+// waves on a SIMD in step overlap little of it.  Reading x a step ahead, or starting every workgroup at another piece, gains
+// nothing.
+constexpr int kW4PieceK = 256, kW4WideWk = 2, kW4WideWc = kW4Waves / kW4WideWk, kW4Ahead = 4;
+constexpr int kW4WideXPitch = kW4PieceK * 2 + 16;
+__host__ __device__ constexpr int w4_wide_x_bytes(int mt) { return 2 * 16 * mt * kW4WideXPitch; }
+
+template <bool F16, int MODE, int RUN, int MT, int KIND, int TN, bool CODES>
+__global__ __launch_bounds__(64 * kW4Waves) void gemm_w4_wide_kernel(W4Args p, int scale_pieces)
+{
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    constexpr bool PER_LANE = RUN == 128 || MODE == kW4Fp4Scaled;
+    constexpr int EB = w4_entry_bytes(MODE, KIND), COLS = 16 * TN * kW4WideWc, UNITS = kW4PieceK / 8;
+    static_assert(16 * MT * UNITS == MT * 64 * kW4Waves, "a thread stages MT pieces of eight numbers");
+    const int lane = threadIdx.x & 63, fi = lane & 15, fq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wc = wave % kW4WideWc, wk = wave / kW4WideWc;
+    const int g = blockIdx.y, n0 = blockIdx.x * COLS;
+    int first, end;
+    w4_group_rows(p, g, first, end);
+    if (end <= first) return;
+    const size_t row_bytes = (size_t)p.k / 2;
+    // (rows past the last column of y, and bytes past the end of the last row, fall outside the extent and read as zeros;
+    // bytes past the end of other rows are the next row's: x is zero there)
+    const __amdgpu_buffer_rsrc_t rw = w4_rsrc(p.w + ((size_t)g * p.n + n0) * row_bytes, (size_t)(p.n - n0 < COLS ? p.n - n0 : COLS) * row_bytes);
+    uint32_t w_at[TN];
+#pragma unroll
+    for (int c = 0; c < TN; ++c) w_at[c] = (uint32_t)(16 * (TN * wc + c) + fi) * (uint32_t)row_bytes + (uint32_t)(wk * (kW4PieceK / kW4WideWk / 2) + fq * 16);
+    const int pieces = (p.k + kW4PieceK - 1) / kW4PieceK;
+    constexpr uint32_t elem = CODES ? 1 : 2;
+    LDS_AS uint8_t *xs = (LDS_AS uint8_t *)lds, *ss = xs + w4_wide_x_bytes(MT);
+    const int x_unit = threadIdx.x % UNITS, x_first = threadIdx.x / UNITS;       // this thread's eight columns and first row of a piece
+    const int runs = scale_pieces * (kW4PieceK / RUN), s_pitch = w4_scale_pitch(runs, EB);
+    const LDS_AS uint8_t *s_lane[TN];
+#pragma unroll
+    for (int c = 0; c < TN; ++c) s_lane[c] = ss + (16 * (TN * wc + c) + fi) * s_pitch + (wk * (kW4PieceK / kW4WideWk / RUN) + (MODE == kW4Fp4Scaled && RUN == 32 ? fq : 0)) * EB;
+    const LDS_AS uint8_t *x_lane = xs + fi * kW4WideXPitch + wk * kW4PieceK + (PER_LANE ? 4 * fq : fq) * 16;
+
+    for (int m0 = first; m0 < end; m0 += 16 * MT) {
+        const int rows = end - m0 < 16 * MT ? end - m0 : 16 * MT;
+        const __amdgpu_buffer_rsrc_t rx = w4_rsrc(static_cast<const uint8_t *>(p.x) + (size_t)m0 * p.k * elem, (size_t)rows * p.k * elem);
+        v4i x_raw[2][MT], w_raw[kW4Ahead][TN];
+        auto load_x = [&](v4i (&r)[MT], int piece) __attribute__((always_inline)) {
+            const int k = piece * kW4PieceK + x_unit * 8;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const uint32_t at = k < p.k ? ((uint32_t)(16 * i + x_first) * (uint32_t)p.k + (uint32_t)k) * elem : 0xFFFFFFF0u;
+                if constexpr (CODES) {
+                    const v2u c = __builtin_amdgcn_raw_buffer_load_b64(rx, (int)at, 0, 0);
+                    r[i] = v4i{(int)c[0], (int)c[1], 0, 0};
+                } else {
+                    r[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rx, (int)at, 0, 0));
+                }
+            }
+        };
+        auto store_x = [&](const v4i (&r)[MT], int buffer) __attribute__((always_inline)) {
+            LDS_AS uint8_t *to = xs + buffer * (16 * MT * kW4WideXPitch) + x_first * kW4WideXPitch + x_unit * 16;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                *reinterpret_cast<LDS_AS v4i *>(to + 16 * i * kW4WideXPitch) = w4_order<MODE>(CODES ? w4_widen(v2u{(uint32_t)r[i][0], (uint32_t)r[i][1]}, p.x_type) : r[i]);
+        };
+        auto load_w = [&](v4i (&r)[TN], int piece) __attribute__((always_inline)) {
+#pragma unroll
+            for (int c = 0; c < TN; ++c)
+                r[c] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, piece < pieces ? (int)(w_at[c] + (uint32_t)piece * (kW4PieceK / 2)) : -16, 0, 2));
+        };
+        v4f total[MT][TN];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int c = 0; c < TN; ++c) total[i][c] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        load_x(x_raw[0], 0);
+#pragma unroll
+        for (int u = 0; u < kW4Ahead; ++u) load_w(w_raw[u], u);
+        __syncthreads();                                  // (the rows before are done with)
+        store_x(x_raw[0], 0);
+        load_x(x_raw[0], 1);
+        load_x(x_raw[1], 2);
+        for (int s0 = 0; s0 < pieces; s0 += scale_pieces) {
+            const int cols = p.n - n0 < COLS ? p.n - n0 : COLS;
+            w4_stage_scales_any<F16, MODE, RUN, KIND>(p, ((size_t)g * p.n + n0) * p.per_row, s0 * kW4PieceK, runs, cols, COLS, ss, threadIdx.x, 64 * kW4Waves);
+            wait_lgkmcnt0();
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            const int s_end = pieces - s0 < scale_pieces ? pieces : s0 + scale_pieces;
+            for (int q0 = s0; q0 < s_end; q0 += kW4Ahead) {
+#pragma unroll
+                for (int u = 0; u < kW4Ahead; ++u) {
+                    const int q = q0 + u;
+                    store_x(x_raw[u & 1], (u + 1) & 1);
+                    __builtin_amdgcn_sched_barrier(0);    // (a load stays behind the last use of its registers: otherwise it gets others, and
+                    load_x(x_raw[u & 1], q + 3);          // the copy back at the end of the loop waits for it)
+                    uint32_t w[TN][4];
+#pragma unroll
+                    for (int c = 0; c < TN; ++c) {
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) w[c][d] = (uint32_t)w_raw[u][c][d];
+                        if constexpr (!PER_LANE) w4_turn(w[c]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    const LDS_AS uint8_t *x_at = x_lane + (u & 1) * (16 * MT * kW4WideXPitch);
+                    const int s_at = (q - s0) * (kW4PieceK / RUN) * EB;
+                    v4f sum[MT][TN];
+                    float s[TN];
+                    v4i minus[TN];
+#pragma unroll
+                    for (int c = 0; c < TN; ++c) {
+                        s[c] = 1.0f;
+                        uint32_t pair = 0;
+                        if constexpr (MODE == kW4Fp4Scaled) w4_entry<MODE, KIND>(s_lane[c] + s_at, s[c], pair);
+                    }
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        const bool open = RUN == 32 || d == 0;         // a new run of the staged scales begins
+                        v4i a[MT];
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) a[i] = *reinterpret_cast<const LDS_AS v4i *>(x_at + 16 * i * kW4WideXPitch + (PER_LANE ? d : 4 * d) * 16);
+#pragma unroll
+                        for (int c = 0; c < TN; ++c) {
+                            if constexpr (MODE != kW4Fp4Scaled)
+                                if (open) {
+                                    uint32_t pair = 0;
+                                    w4_entry<MODE, KIND>(s_lane[c] + s_at + (RUN == 32 ? d : 0) * EB, s[c], pair);
+                                    minus[c] = v4i{(int)pair, (int)pair, (int)pair, (int)pair};
+                                }
+                            const v4i wide = w4_expand<F16, MODE>(w[c][d], MODE == kW4Fp4Scaled ? s[c] : 1.0f);
+#pragma unroll
+                            for (int i = 0; i < MT; ++i) {
+                                if constexpr (MODE == kW4Fp4Scaled) {
+                                    total[i][c] = w4_mfma<F16>(a[i], wide, total[i][c]);
+                                } else {
+                                    sum[i][c] = w4_mfma<F16>(a[i], wide, open ? v4f{0.0f, 0.0f, 0.0f, 0.0f} : sum[i][c]);
+                                }
+                            }
+                            if constexpr (MODE == kW4Int)
+#pragma unroll
+                                for (int i = 0; i < MT; ++i) sum[i][c] = w4_mfma<F16>(a[i], minus[c], sum[i][c]);
+                        }
+                        if (MODE != kW4Fp4Scaled && (RUN == 32 || d == 3)) {
+#pragma unroll
+                            for (int c = 0; c < TN; ++c)
+#pragma unroll
+                                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                                    for (int r = 0; r < 4; ++r) total[i][c][r] += s[c] * sum[i][c][r];
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    load_w(w_raw[u], q + kW4Ahead);
+                    wait_lgkmcnt0();
+                    asm volatile("" ::: "memory");
+                    __builtin_amdgcn_s_barrier();         // (the loads in flight go on)
+                    asm volatile("" ::: "memory");
+                }
+            }
+        }
+        // ---- the two waves along K; register r of lane (fi, fq) holds y[16 i + 4 fq + r][column fi]
+        LDS_AS float *part = (LDS_AS float *)xs + wc * (TN * MT * 256);
+        if (wk == 1) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int c = 0; c < TN; ++c) *reinterpret_cast<LDS_AS v4f *>(part + ((i * TN + c) * 64 + lane) * 4) = total[i][c];
+        }
+        __syncthreads();
+        if (wk == 0) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int c = 0; c < TN; ++c) {
+                    const v4f other = *reinterpret_cast<const LDS_AS v4f *>(part + ((i * TN + c) * 64 + lane) * 4);
+                    const int col = n0 + 16 * (TN * wc + c) + fi;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int row = i * 16 + 4 * fq + r;
+                        if (row < rows && col < p.n)
+                            store_out(p.y, (size_t)(m0 + row) * p.n + col, (total[i][c][r] + other[r]) * (p.x_scale ? p.x_scale[m0 + row] : 1.0f), p.y_type);
+                    }
+                }
         }
     }
 }

@@ -12,17 +12,17 @@
 
 namespace fp8gemm_detail {
 
-template <bool F16, int MODE, int RUN, int MT, int KIND>
+template <bool F16, int MODE, int RUN, int KIND>
 struct W4KernelTag {};
 
 constexpr int kW4MaxLds = 160 * 1024;
 
-template <bool F16, int MODE, int RUN, int MT, int KIND>
+template <bool F16, int MODE, int RUN, int KIND>
 hipError_t launch_w4_kernel(W4Args p, hipStream_t s)
 {
     // Rows of x that an expert has at a time, as far as the host can tell.
     const int busy = std::min(p.rows, p.groups);
-    const int rows = std::min((p.rows + busy - 1) / busy, 16 * MT);
+    const int rows = std::min((p.rows + busy - 1) / busy, 16);
     const long col_tiles = (p.n + 15) / 16, row_bytes = p.k / 2;
     // How the eight waves are laid out, how many workgroups share a CU and how many blocks of columns each takes: the
     // least time in units of one ring stage of a workgroup -- half a unit to add the waves along K up, six to
@@ -32,8 +32,8 @@ hipError_t launch_w4_kernel(W4Args p, hipStream_t s)
     constexpr int EB = w4_entry_bytes(MODE, KIND);
     double best = 1e30;
     int best_lds = 0;
-    p.part_rows = std::min(p.rows, 16 * MT);
-    for (int per_cu = MT == 1 ? 2 : 1; per_cu >= 1; --per_cu)
+    p.part_rows = std::min(p.rows, 16);
+    for (int per_cu = 2; per_cu >= 1; --per_cu)
         for (int wk = 1; wk <= kW4Waves; wk *= 2) {
             if (wk > 1 && p.k <= (wk - 1) * kW4StageK) continue;
             const int wc = kW4Waves / wk, unit = kW4StageK * wk, slot = w4_ring_bytes(1);
@@ -67,21 +67,56 @@ hipError_t launch_w4_kernel(W4Args p, hipStream_t s)
         }
     if (best_lds == 0) return hipErrorInvalidValue;
     const int lds = best_lds, wc = kW4Waves >> p.wk_shift;
-    auto kernel = gemv_w4_kernel<F16, MODE, RUN, MT, KIND>;
-    hipError_t e = allow_lds<W4KernelTag<F16, MODE, RUN, MT, KIND>>(kernel, kW4MaxLds);
+    auto kernel = gemv_w4_kernel<F16, MODE, RUN, KIND>;
+    hipError_t e = allow_lds<W4KernelTag<F16, MODE, RUN, KIND>>(kernel, kW4MaxLds);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kernel, dim3((unsigned)((col_tiles + wc * p.blocks - 1) / (wc * p.blocks)), (unsigned)p.groups), dim3(64 * kW4Waves), lds, s, p);
     return hipGetLastError();
 }
 
+template <bool F16, int MODE, int RUN, int MT, int KIND, int TN, bool CODES>
+struct W4WideKernelTag {};
+
+template <bool F16, int MODE, int RUN, int MT, int KIND, int TN, bool CODES>
+hipError_t launch_w4_wide(const W4Args &p, hipStream_t s)
+{
+    constexpr int COLS = 16 * TN * kW4WideWc, EB = w4_entry_bytes(MODE, KIND), ROOM = kW4MaxLds - w4_wide_x_bytes(MT);
+    // the scales of all of K, or of equal parts, whole turns of the weights' registers
+    const int pieces = (p.k + kW4PieceK - 1) / kW4PieceK;
+    auto bytes = [](int pieces_) { return COLS * w4_scale_pitch(pieces_ * (kW4PieceK / RUN), EB); };
+    static_assert(COLS * w4_scale_pitch(kW4Ahead * (kW4PieceK / RUN), EB) <= ROOM, "no room for the scales");
+    int parts = 1, scale_pieces;
+    do {
+        scale_pieces = ((pieces + parts - 1) / parts + kW4Ahead - 1) / kW4Ahead * kW4Ahead;
+        ++parts;
+    } while (bytes(scale_pieces) > ROOM);
+    auto kernel = gemm_w4_wide_kernel<F16, MODE, RUN, MT, KIND, TN, CODES>;
+    hipError_t e = allow_lds<W4WideKernelTag<F16, MODE, RUN, MT, KIND, TN, CODES>>(kernel, kW4MaxLds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((p.n + COLS - 1) / COLS), (unsigned)p.groups), dim3(64 * kW4Waves), w4_wide_x_bytes(MT) + bytes(scale_pieces), s, p, scale_pieces);
+    return hipGetLastError();
+}
+
+template <bool F16, int MODE, int RUN, int MT, int KIND>
+hipError_t launch_w4_tall(const W4Args &p, int busy, hipStream_t s)
+{
+    // Two blocks of 16 columns a wave where workgroups of 128 columns still keep half the CUs busy (us for one / two: 32 x
+    // 4096 x 4096 15.2 / 21.8, 64 x 4096 x 16384 22.3 / 28.2, 48 x 2048 x 24576 33.3 / 29.1, 17 x 8192 x 28672 49.0 / 40.7).
+    const bool wide = (long)(p.n + 127) / 128 * busy > 128;
+    if constexpr (F16)
+        if (p.x_type != FP8GEMM_T_F16)
+            return wide ? launch_w4_wide<F16, MODE, RUN, MT, KIND, 2, true>(p, s) : launch_w4_wide<F16, MODE, RUN, MT, KIND, 1, true>(p, s);
+    return wide ? launch_w4_wide<F16, MODE, RUN, MT, KIND, 2, false>(p, s) : launch_w4_wide<F16, MODE, RUN, MT, KIND, 1, false>(p, s);
+}
+
 template <bool F16, int MODE, int RUN, int KIND>
 hipError_t launch_w4_rows(const W4Args &p, hipStream_t s)
 {
-    // rows of x per pass over the weights; with experts, what an expert has on average
-    const int average = (p.rows + p.groups - 1) / p.groups;
-    if (p.rows <= 16 || average <= 8) return launch_w4_kernel<F16, MODE, RUN, 1, KIND>(p, s);
-    if (p.rows <= 32 || average <= 16) return launch_w4_kernel<F16, MODE, RUN, 2, KIND>(p, s);
-    return launch_w4_kernel<F16, MODE, RUN, 4, KIND>(p, s);
+    // Rows of x per pass over the weights; with experts, what an expert has on average (eight experts, us for gemv / 32 rows at a
+    // time: 4096 x 4096 integers, 8 rows each 23.2 / 25.2, 12 rows 30.6 / 25.1; 2048 x 2048 e2m1, 8 rows 16.2 / 9.9).
+    const int busy = std::min(p.rows, p.groups), average = (p.rows + busy - 1) / busy;
+    if (p.rows <= 16 || average <= 6) return launch_w4_kernel<F16, MODE, RUN, KIND>(p, s);
+    return p.rows <= 32 || average <= 16 ? launch_w4_tall<F16, MODE, RUN, 2, KIND>(p, busy, s) : launch_w4_tall<F16, MODE, RUN, 4, KIND>(p, busy, s);
 }
 
 template <bool F16, int MODE>

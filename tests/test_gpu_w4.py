@@ -79,6 +79,62 @@ def test_lengths(pkg, k, n, m):
             run_case(pkg, m, k, n, 128, w_fmt, torch.float16, False, torch.float16, torch.float32, "lengths")
 
 
+@pytest.mark.parametrize("w_fmt", [0, 1])
+@pytest.mark.parametrize("scale", SCALES)
+@pytest.mark.parametrize("x_type", XS)
+@pytest.mark.parametrize("m", [20, 50])
+@pytest.mark.parametrize("run", [32, 128])
+def test_types_with_many_rows(pkg, w_fmt, scale, x_type, m, run):
+    """The kernel for more rows of x, one and two blocks of columns a wave (which one: n)."""
+    run_case(pkg, m, 768, 40, run, w_fmt, scale, w_fmt == 0, x_type, torch.float32, "many")
+    run_case(pkg, m, 384, 16900, run, w_fmt, scale, w_fmt == 0, x_type, torch.bfloat16, "many")
+
+
+@pytest.mark.parametrize("k", [32, 64, 256, 288, 1056, 2048, 8192, 28672])
+@pytest.mark.parametrize("m,n", [(17, 1), (32, 200), (64, 129), (130, 63)])
+def test_lengths_with_many_rows(pkg, k, m, n):
+    """K from a part of a piece to scales that are staged in several parts."""
+    for w_fmt in (0, 1):
+        run_case(pkg, m, k, n, 32, w_fmt, torch.float32, w_fmt == 0, torch.bfloat16, torch.float32, "lengths")
+        if k % 128 == 0:
+            run_case(pkg, m, k, n, 128, w_fmt, torch.float16, False, torch.float16, torch.float32, "lengths")
+
+
+@pytest.mark.parametrize("counts", [[33, 0, 1, 20], [200, 0, 7], [16, 17, 15, 32, 31], [129, 64]])
+@pytest.mark.parametrize("w_fmt,run,scale,x_type", [(0, 128, torch.float16, torch.float16), (1, 32, torch.uint8, torch.bfloat16), (0, 64, torch.bfloat16, F8[1]), (1, 32, torch.float32, F8[0])])
+def test_experts_with_many_rows(pkg, counts, w_fmt, run, scale, x_type):
+    """Passes over more rows than are held at once; rows in front of the first expert and behind the last stay."""
+    gen = generator("many", counts, run)
+    e, n, k = len(counts), 150, 1152
+    w, s, z = weights(gen, (e,), n, k, run, w_fmt, scale, w_fmt == 0)
+    m = sum(counts) + 5
+    off = offsets_of(counts, 2)
+    x = torch.randn((m, k), generator=gen, device="cuda").to(x_type)
+    y = torch.full((m, n), 9.0, device="cuda")
+    pkg.gemv_w4(x, w, s, run, w_fmt=w_fmt, zeros=z, row_offsets=off, out=y)
+    for g in range(e):
+        lo, hi = int(off[g]), int(off[g + 1])
+        if hi > lo:
+            ref = x[lo:hi].double() @ w4_values(w[g], s[g], run, w_fmt, None if z is None else z[g]).t().contiguous()
+            bound = (62.0 if w_fmt == 0 else 6.0) * scale_values(s[g]).repeat_interleave(run, -1)
+            assert ((y[lo:hi].double() - ref).abs() <= tolerance(x[lo:hi].double(), None, bound, torch.float32, ref)).all()
+    assert (y[:2] == 9.0).all() and (y[int(off[e]):] == 9.0).all()
+
+
+def test_operands_that_end_with_their_memory(pkg):
+    """What lies behind x and W, NaNs here, stays out of the results (a K that ends inside a piece)."""
+    gen = generator("end")
+    for m in (3, 20, 50):
+        for k, n in ((288, 33), (32, 65), (1056, 150)):
+            w, s, z = weights(gen, (), n, k, 32, 0, torch.float16, True)
+            x = torch.randn((m, k), generator=gen, device="cuda").to(torch.bfloat16)
+            want = pkg.gemv_w4(x, w, s, 32, zeros=z)
+            store = torch.full((m * k + 4096,), float("nan"), dtype=torch.bfloat16, device="cuda")
+            x2 = store[:m * k].view(m, k).copy_(x)
+            s2 = torch.full((s.numel() + 4096,), float("nan"), dtype=s.dtype, device="cuda")[:s.numel()].view(s.shape).copy_(s)
+            assert torch.equal(pkg.gemv_w4(x2, w, s2, 32, zeros=z), want)
+
+
 @pytest.mark.parametrize("x_type", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("run", [32, 128])
 def test_every_nibble_in_every_place(pkg, x_type, run):
