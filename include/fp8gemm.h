@@ -294,8 +294,8 @@ int fp8gemm_launch_algo(int m, int k, int n, const void *a, int a_fmt, const voi
 int fp8gemm_launch_tuned(int m, int k, int n, const void *a, int a_fmt, const void *b, int b_fmt,
                          float *out, int algo, int variant, int split_k, void *stream);
 int fp8gemm_num_variants(int algo);
-/* fp8gemm_grouped / fp8gemm_grouped_wgrad on one of their kernels: 0 the one for any shape (grouped only), 13 and 18
- * tile shapes of both, 14, 15, 17 and 19 of the first; -1 = the plan's choice.  hipErrorInvalidValue where the kernel cannot run the shape. */
+/* fp8gemm_grouped / fp8gemm_grouped_wgrad on one of their kernels: 0 the one for any shape (grouped only), 13, 15,
+ * 18 and 19 tile shapes of both, 14 and 17 of the first; -1 = the plan's choice.  hipErrorInvalidValue where the kernel cannot run the shape. */
 int fp8gemm_grouped_tuned(int groups, int m, int k, int n, const int *row_offsets, const void *a, int a_fmt, const void *b, int b_fmt,
                           void *out, int out_type, const float *a_scale, const float *b_scale, int b_scale_per_column, int variant,
                           void *stream);

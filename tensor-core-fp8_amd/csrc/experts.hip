@@ -70,13 +70,34 @@ int plan_grouped(int m, int k, int n, int groups)
     return pick;
 }
 
-// The weight gradient: the 256 x 256 tile on the 16x16x128 MFMA once an expert has some four K tiles of tokens, below
-// that the 128 x 128 tile with two workgroups on a CU, whose epilogues overlap (bf16 output, us, 128 x 128 / 256 x 256: 16 experts
-// of 2048 x 1024, 128 tokens each 24.3 / 27.1, 512 33.5 / 35.1, 2048 85.7 / 79.7; 4 of 8192 x 4096, 256 tokens 98.9 / 101.7, 512
-// 122.8 / 115.4, 4096 524 / 396; 128 x 256 and 192 x 256 tiles lie behind one of the two everywhere).
-int plan_wgrad(int rows, int groups)
+// The weight gradient: the same model, with the bytes of C alone (every other one is read for a tile's K walk).  Fitted to 114 cuts
+// (1 to 16 experts, 128 to 32768 rows, m and n 256 to 8192): the pick takes 0.6 % longer than the best of the four on
+// average.  One tile shape for all: us of 13 / 18 / 19 / 15 for one expert of 16384 rows, 512 x 1024, 139 / 70 / 45 / 41, 4096 x 4096
+// 174 / 242 / 332 / 338; for 16 experts of 131 rows, 2048 x 2048, 51 / 46 / 60 / 91.
+constexpr GroupedCost kWgradCosts[] = {
+    {13, 256, 256, 1, true, 1.327, 9.87, 6.4e7, 0.733},
+    {18, 128, 128, 2, true, 0.913, 3.28, 3.39e6, 0.399},
+    {19, 64, 128, 2, true, 0.668, 2.45, 2.53e6, 0.394},
+    {15, 64, 128, 1, true, 0.337, 2.30, 1e9, 0.780},
+};
+
+int plan_wgrad(int rows, int m, int n, int groups)
 {
-    return rows / groups < 512 ? 18 : 13;
+    const double kt = groups == 1 ? (rows + 127) / 128 : (double)rows / groups / 128 + 0.5;
+    int pick = 18;
+    double best = 1e30;
+    for (const GroupedCost &c : kWgradCosts) {
+        const double rounds = (double)groups * ((m + c.bm - 1) / c.bm) * ((n + c.bn - 1) / c.bn) / (256.0 * c.per_cu);
+        const double whole = std::floor(rounds), rest = rounds - whole, tiles = c.variant == 13 ? std::max(kt, 2.0) : kt;
+        double cost = whole * (tiles * c.per_k_tile + c.per_item);
+        if (rest > 1e-9) cost += tiles * c.per_k_tile * (c.idle + (1.0 - c.idle) * rest) + c.per_item;
+        cost = std::max(cost, 2.0 * groups * m * n / c.stream_rate);
+        if (cost < best) {
+            best = cost;
+            pick = c.variant;
+        }
+    }
+    return pick;
 }
 
 }  // namespace fp8gemm_detail

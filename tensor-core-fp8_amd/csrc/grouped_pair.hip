@@ -77,10 +77,12 @@ hipError_t dispatch_grouped(int m, int k, int n, const uint8_t *a, const uint8_t
 template <int AF, int BF>
 hipError_t dispatch_wgrad(int m, int ld, int n, const uint8_t *a_t, const uint8_t *b_t, void *out, int variant, const GroupSpec &grp, hipStream_t stream)
 {
-    if (variant < 0) variant = plan_wgrad(grp.rows, grp.groups);
+    if (variant < 0) variant = plan_wgrad(grp.rows, m, n, grp.groups);
     switch (variant) {
     case 13: return launch_grouped_shape<TileP2h, AF, BF, false, false, false, kGroupedK, 1>(m, ld, n, a_t, b_t, out, 2, grp, stream);
     case 18: return launch_grouped_shape<TileQ2, AF, BF, false, false, false, kGroupedK, 2>(m, ld, n, a_t, b_t, out, 2, grp, stream);
+    case 19: return launch_grouped_shape<TileE3, AF, BF, false, false, false, kGroupedK, 2>(m, ld, n, a_t, b_t, out, 2, grp, stream);
+    case 15: return launch_grouped_shape<TileE5, AF, BF, false, false, true, kGroupedK, 1>(m, ld, n, a_t, b_t, out, 2, grp, stream);
     default: return hipErrorInvalidValue;
     }
 }

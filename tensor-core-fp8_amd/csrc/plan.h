@@ -107,7 +107,7 @@ hipError_t dispatch_bell(int m, int kell, int n, const uint8_t *values, const ui
 // Products grouped by expert: tile shapes by the numbers above, or the kernel for any shape.
 constexpr int kGroupedDirect = 0;
 int plan_grouped(int m, int k, int n, int groups);
-int plan_wgrad(int rows, int groups);
+int plan_wgrad(int rows, int m, int n, int groups);
 // variant < 0: the plan's choice.  grouped: rows of A and C cut among the groups; wgrad: K (the tokens, row stride ld).
 template <int AF, int BF>
 hipError_t dispatch_grouped(int m, int k, int n, const uint8_t *a, const uint8_t *b, void *out, int variant, const GroupSpec &grp, hipStream_t stream);

@@ -285,7 +285,7 @@ def test_wgrad_every_kernel(pkg, variant, counts, m, n):
 
 
 @pytest.mark.parametrize("fa,fb", PAIRS)
-@pytest.mark.parametrize("variant", [13, 18])
+@pytest.mark.parametrize("variant", [13, 15, 18, 19])
 def test_wgrad_pairings(pkg, fa, fb, variant):
     gen = generator("wgrad pairs", fa, fb)
     off, a, at, cs = transposed(gen, [129, 2, 500], 192, fa)
@@ -300,7 +300,7 @@ def test_wgrad_many_tiles_per_workgroup(pkg):
     counts = [1500, 0, 7, 300, 1]
     off, a, at, cs = transposed(gen, counts, 2100, 0)
     _, b, _, _ = transposed(gen, counts, 1900, 0)
-    for variant in (13, 18):
+    for variant in (13, 15, 18, 19):
         out = pkg.gemm_grouped_wgrad(a, b, off, sum(counts), variant=variant)
         for g, (p, c) in enumerate(zip(at, cs)):
             if not c:
@@ -316,7 +316,7 @@ def test_wgrad_captured_and_replayed(pkg):
     counts = [200, 0, 56]
     off, a, at, cs = transposed(gen, counts, 128, 0)
     _, b, _, _ = transposed(gen, counts, 256, 0)
-    for variant in (13, 18):
+    for variant in (13, 15, 18, 19):
         out = torch.zeros((3, 128, 256), device="cuda")
         pkg.gemm_grouped_wgrad(a, b, off, 256, out=out, variant=variant)
         graph = torch.cuda.CUDAGraph()
@@ -344,7 +344,7 @@ def test_wgrad_operands_that_end_with_their_memory(pkg):
         one = torch.tensor([0, sum(counts)], dtype=torch.int32, device="cuda")
         pick = torch.randint(0, 16384, (64,), generator=gen, device="cuda")
         y, tol = fp8_product(a.float()[pick].double(), b.double())
-        for variant in (13, 18):
+        for variant in (13, 15, 18, 19):
             check(pkg.gemm_grouped_wgrad(a, b, one, rows, variant=variant)[0][pick], y, tol + rounding(y, torch.float32) * 1.0001)
 
 
@@ -355,7 +355,7 @@ def test_wgrad_many_experts_and_results_beyond_31_bits(pkg):
         counts[g] = c
     off, a, at, cs = transposed(gen, counts, 2048, 0)
     _, b, _, _ = transposed(gen, counts, 1152, 0)
-    for variant in (13, 18):
+    for variant in (13, 15, 18, 19):
         out = torch.full((1024, 2048, 1152), 5.0, dtype=torch.bfloat16, device="cuda")
         assert out.numel() > 2 ** 31
         pkg.gemm_grouped_wgrad(a, b, off, sum(counts), out=out, variant=variant)
@@ -372,7 +372,7 @@ def test_wgrad_output_anywhere(pkg, dtype):
     off, a, at, cs = transposed(gen, [100, 0, 30], 130, 0)
     _, b, _, _ = transposed(gen, [100, 0, 30], 68, 0)
     size = 3 * 130 * 68
-    for variant in (13, 18):
+    for variant in (13, 15, 18, 19):
         for shift in (1, 3):
             store = torch.full((size + 16,), 3.0, dtype=dtype, device="cuda")
             out = store[shift:shift + size].view(3, 130, 68)
