@@ -164,7 +164,6 @@ template <int TYPE, int FMT>
 hipError_t launch_quantize_rows(int rows, int cols, const void *x, size_t stride, int x_rows, const int *index, uint8_t *codes, float *scales, hipStream_t s)
 {
     const size_t elem = TYPE == FP8GEMM_OUT_F32 ? 4 : 2;
-    const bool vec = cols % 8 == 0 && aligned_to(x, 16) && stride * elem % 16 == 0 && aligned_to(codes, 8);
     for (; rows > 0; rows -= kRowsAtOnce) {
         const int now = std::min(rows, kRowsAtOnce);
 #define ROWS_KERNEL(WAVES, HELD)                                                                                                            \
@@ -173,11 +172,11 @@ hipError_t launch_quantize_rows(int rows, int cols, const void *x, size_t stride
         // Four waves to a row, two or eight pieces of eight elements a lane; short rows get a wave each, for which four would be
         // half idle.  One wave with eight pieces for rows of 4096 is slower: 32768 rows 109 us against 97, 3001 rows of
         // 2048 11.6 against 9.8 (other data read in between, so that x is not cached).
-        if (vec && cols <= 1024)
+        if (cols <= 1024)
             ROWS_KERNEL(1, 2);
-        else if (vec && cols <= 4096)
+        else if (cols <= 4096)
             ROWS_KERNEL(4, 2);
-        else if (vec && cols <= 16384)
+        else if (cols <= 16384)
             ROWS_KERNEL(4, 8);
         else
             hipLaunchKernelGGL((quantize_rows_any_kernel<TYPE, FMT>), dim3((unsigned)now), dim3(256), 0, s, cols, x, stride, x_rows, index, codes, scales);
@@ -200,17 +199,25 @@ template <int TYPE, int FMT>
 hipError_t launch_quantize_columns(const GroupSpec &grp, int cols, const void *x, size_t stride, int x_rows, const int *index, uint8_t *codes, size_t ld,
                                    float *scales, hipStream_t s)
 {
-    const size_t elem = TYPE == FP8GEMM_OUT_F32 ? 4 : 2;
-    const bool vec = cols % 8 == 0 && aligned_to(x, 16) && stride * elem % 16 == 0;
     const long col_blocks = (cols + kColBlock - 1) / kColBlock;
-    const long grid = col_blocks * (grp.groups + 1);
-    if (grid > 0xFFFFFFFFL / kColThreads) return hipErrorInvalidValue;
-    if (vec)
-        hipLaunchKernelGGL((quantize_columns_kernel<TYPE, FMT, true>), dim3((unsigned)grid), dim3(kColThreads), 0, s, grp, cols, x, stride, x_rows, index, codes, ld,
-                           scales);
-    else
-        hipLaunchKernelGGL((quantize_columns_kernel<TYPE, FMT, false>), dim3((unsigned)grid), dim3(kColThreads), 0, s, grp, cols, x, stride, x_rows, index, codes, ld,
-                           scales);
+#define COLUMNS_KERNEL(PART, WORKGROUPS)                                                                                                             \
+    hipLaunchKernelGGL((quantize_columns_kernel<TYPE, FMT, PART>), dim3((unsigned)(WORKGROUPS)), dim3(kColThreads), 0, s, grp, cols, x, stride, x_rows, index, \
+                       codes, ld, scales)
+    const int busy = std::min(grp.rows, grp.groups);
+    const long batches = grp.rows / col_rows(TYPE) + grp.groups;          // as many as any cut of the rows has
+    if (col_blocks * std::max(batches, (long)grp.groups) > 0xFFFFFFFFL / kColThreads - col_blocks) return hipErrorInvalidValue;
+    // Split over the rows where the whole walks leave CUs idle and take several batches (bf16, us split / whole: one expert of 16384
+    // rows, 512 columns 22 / 144, 2000 rows 17.7 / 21.2; 3 of 2667, 2048 columns 29 / 48; but one of 1500, 4096 columns 20.6 / 18.6, 16 of
+    // 512, 2048 columns 31 / 23, 32 of 1024, 4096 columns 186 / 120).
+    if (col_blocks * busy < 256 && grp.rows / busy > 3 * col_rows(TYPE)) {
+        const size_t count = (size_t)grp.groups * cols;
+        hipLaunchKernelGGL(quantize_clear_kernel, dim3((unsigned)((count + 255) / 256)), dim3(256), 0, s, scales, count);
+        COLUMNS_KERNEL(kColMaxima, col_blocks * batches);
+        COLUMNS_KERNEL(kColCodes, col_blocks * (batches + 1));
+    } else {
+        COLUMNS_KERNEL(kColWhole, col_blocks * (grp.groups + 1));
+    }
+#undef COLUMNS_KERNEL
     return hipGetLastError();
 }
 

@@ -50,20 +50,44 @@ __device__ __forceinline__ uint32_t quant_four(float a, float b, float c, float 
     return w;
 }
 
-// eight consecutive elements as they are stored (a 16-bit type fills the first half)
+// Eight consecutive elements as they are stored (a 16-bit type fills the first half), from any element's place: global memory
+// takes 16 bytes at once from every address, only lines that are touched twice cost something.
+typedef int quant_v4i __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t quant_v2u __attribute__((ext_vector_type(2), aligned(1)));
 struct QuantRaw {
     v4i lo, hi;
 };
 template <int TYPE>
-__device__ __forceinline__ QuantRaw quant_load8_raw(const void *base, size_t index)      // from a 16-byte aligned place
+__device__ __forceinline__ QuantRaw quant_load8_raw(const void *base, size_t index)
 {
     QuantRaw r = {{0, 0, 0, 0}, {0, 0, 0, 0}};
     if (TYPE == FP8GEMM_DEV_OUT_F32) {
-        const v4i *p = reinterpret_cast<const v4i *>(static_cast<const float *>(base) + index);
+        const quant_v4i *p = reinterpret_cast<const quant_v4i *>(static_cast<const float *>(base) + index);
         r.lo = p[0];
         r.hi = p[1];
     } else {
-        r.lo = *reinterpret_cast<const v4i *>(static_cast<const unsigned short *>(base) + index);
+        r.lo = *reinterpret_cast<const quant_v4i *>(static_cast<const unsigned short *>(base) + index);
+    }
+    return r;
+}
+// the first `count` < 8 of them, zeros behind
+template <int TYPE>
+__device__ __forceinline__ QuantRaw quant_load_some(const void *base, size_t index, int count)
+{
+    QuantRaw r = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+    for (int i = 0; i < 7; ++i) {
+        if (i >= count) continue;
+        if (TYPE == FP8GEMM_DEV_OUT_F32) {
+            const int w = static_cast<const int *>(base)[index + i];
+            if (i < 4)
+                r.lo[i & 3] = w;
+            else
+                r.hi[i & 3] = w;
+        } else {
+            const uint32_t h = static_cast<const unsigned short *>(base)[index + i];
+            r.lo[i / 2] = (int)((uint32_t)r.lo[i / 2] | (h << (16 * (i & 1))));
+        }
     }
     return r;
 }
@@ -85,13 +109,6 @@ __device__ __forceinline__ void quant_unpack8(const QuantRaw &r, float v[8])
         }
     }
 }
-template <int TYPE>
-__device__ __forceinline__ void quant_load8(const void *base, size_t index, float v[8])
-{
-    const QuantRaw r = quant_load8_raw<TYPE>(base, index);
-    quant_unpack8<TYPE>(r, v);
-}
-
 // folds |x| into the running maximum of finite magnitudes; whether x is an infinity or a NaN
 __device__ __forceinline__ bool quant_fold(float x, uint32_t &amax_bits)
 {
@@ -104,7 +121,7 @@ __device__ __forceinline__ bool quant_fold(float x, uint32_t &amax_bits)
 // Row r of codes = row (row_index ? row_index[r] : r) of x; a row_index outside [0, x_rows) gives a row of zeros with
 // scale 1.  WAVES waves to a row, 4 / WAVES rows to a workgroup.  HBM bound: every wide element is read once, held in
 // registers (HELD pieces of eight elements a lane) until the row's maximum is known, and its code written: 32768 rows
-// of 4096 bf16 gathered from 16384 take 74 us.
+// of 4096 bf16 take 70 us, gathered from 16384 74, 8192 rows of 1843 16.5.
 template <int TYPE, int FMT, int WAVES, int HELD>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(int rows, int cols, const void *__restrict__ x, size_t x_stride, int x_rows,
                                                             const int *__restrict__ row_index, uint8_t *__restrict__ codes, float *__restrict__ scales)
@@ -123,11 +140,15 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(int rows, int cols, 
 #pragma unroll
     for (int h = 0; h < HELD; ++h) {
         const int c = ((h * WAVES + sub) * 64 + lane) * 8;
-        if (there && c < cols) {
-            quant_load8<TYPE>(x, (size_t)src * x_stride + c, v[h]);
-        } else {
+        QuantRaw raw = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        if (there && c + 8 <= cols) raw = quant_load8_raw<TYPE>(x, (size_t)src * x_stride + c);
+        quant_unpack8<TYPE>(raw, v[h]);
+    }
+    if (cols % 8 != 0) {                                   // the last piece of a row is a part of one
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[h][i] = 0.0f;
+        for (int h = 0; h < HELD; ++h) {
+            const int c = ((h * WAVES + sub) * 64 + lane) * 8;
+            if (there && c < cols && c + 8 > cols) quant_unpack8<TYPE>(quant_load_some<TYPE>(x, (size_t)src * x_stride + c, cols - c), v[h]);
         }
     }
 #pragma unroll
@@ -161,13 +182,17 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(int rows, int cols, 
             v2u w;
             w[0] = quant_four<FMT>(v[h][0] * inv, v[h][1] * inv, v[h][2] * inv, v[h][3] * inv, rough);
             w[1] = quant_four<FMT>(v[h][4] * inv, v[h][5] * inv, v[h][6] * inv, v[h][7] * inv, rough);
-            *reinterpret_cast<v2u *>(codes + (size_t)row * cols + c) = w;
+            uint8_t *to = codes + (size_t)row * cols + c;
+            if (c + 8 <= cols)
+                *reinterpret_cast<quant_v2u *>(to) = w;
+            else
+                for (int i = 0; i < cols - c; ++i) to[i] = (uint8_t)(w[i / 4] >> (8 * (i & 3)));
         }
     }
     if (lane == 0 && sub == 0) scales[row] = quant_scale(e);
 }
 
-// The same for any row length, stride and alignment: a workgroup to a row, which is read twice.
+// The same for any row length: a workgroup to a row, which is read twice.
 template <int TYPE, int FMT>
 __global__ __launch_bounds__(256) void quantize_rows_any_kernel(int cols, const void *__restrict__ x, size_t x_stride, int x_rows,
                                                                 const int *__restrict__ row_index, uint8_t *__restrict__ codes, float *__restrict__ scales)
@@ -214,40 +239,27 @@ __global__ __launch_bounds__(256) void quantize_rows_any_kernel(int cols, const 
 // columns (a line of 16-bit numbers) of one group, 256 or 512 rows at a time, quads of rows of eight columns a thread: a first walk
 // finds the maxima, the second one goes backwards, so that it starts with the rows that are still in registers (all of
 // them, for a group of no more rows) and goes on with those that are still cached.  128 x 64 pieces are turned
-// around in LDS, so that every column's 128 codes leave as one whole line.
+// around in LDS, so that every column's 128 codes leave as one whole line.  32768 rows of 4096 bf16 in 32 groups: 120 us, 3.4 TB/s
+// (half of the rows are read a second time), 4099 rows of 2048 in 8: 16.
 constexpr int kColBlock = 64;
 constexpr int kColThreads = 512;
 // rows at a time: four or eight a thread, which are 32 registers of either
 __host__ __device__ constexpr int col_rows(int type) { return kColThreads / 8 * (type == FP8GEMM_DEV_OUT_F32 ? 4 : 8); }
 constexpr int kColPitch = kTokenRun + 4;       // bytes of a column in LDS: 33 words, so that eight columns x eight words hit 64 banks
 
-// elements at + c .. at + c + 7, those from `cols` on as zeros
-template <int TYPE, bool VEC>
-__device__ __forceinline__ QuantRaw quant_load_cols(const void *x, size_t at, int c, int cols)
+// Where few blocks of columns and few groups leave CUs without work, the walks are split over the rows: a kernel for the
+// maxima (PART 1: a workgroup takes the rows of one batch and raises the scales, cleared before, to its own -- a power of two
+// orders like its bits, so the order of the workgroups does not matter) and one for the codes (PART 2).  16384 rows of 512 columns
+// of one group take 22 us, in one walk 144.
+constexpr int kColWhole = 0, kColMaxima = 1, kColCodes = 2;
+
+__global__ __launch_bounds__(256) void quantize_clear_kernel(float *scales, size_t count)
 {
-    QuantRaw r = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-    if (VEC) {
-        if (c < cols) r = quant_load8_raw<TYPE>(x, at + c);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (c + i >= cols) continue;
-            if (TYPE == FP8GEMM_DEV_OUT_F32) {
-                const int w = static_cast<const int *>(x)[at + c + i];
-                if (i < 4)
-                    r.lo[i & 3] = w;
-                else
-                    r.hi[i & 3] = w;
-            } else {
-                const uint32_t h = static_cast<const unsigned short *>(x)[at + c + i];
-                r.lo[i / 2] = (int)((uint32_t)r.lo[i / 2] | (h << (16 * (i & 1))));
-            }
-        }
-    }
-    return r;
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < count) scales[i] = 0.0f;
 }
 
-template <int TYPE, int FMT, bool VEC>
+template <int TYPE, int FMT, int PART>
 __global__ __launch_bounds__(kColThreads) void quantize_columns_kernel(GroupSpec grp, int cols, const void *__restrict__ x, size_t x_stride, int x_rows,
                                                                        const int *__restrict__ row_index, uint8_t *__restrict__ codes_t, size_t ld,
                                                                        float *__restrict__ scales)
@@ -255,12 +267,27 @@ __global__ __launch_bounds__(kColThreads) void quantize_columns_kernel(GroupSpec
     using lds_int = __attribute__((address_space(3))) int;
     constexpr int WAVES = kColThreads / 64, ROWS = col_rows(TYPE), RUNS = ROWS / kTokenRun, QUADS = ROWS / (kColThreads / 2);
     __shared__ int table[2 * (kMaxGroups + 1)];
+    __shared__ int batch_table[PART == kColWhole ? 1 : kMaxGroups + 1];
     __shared__ uint32_t amax_of[WAVES][kColBlock];
-    __shared__ uint8_t turn[RUNS][kColBlock * kColPitch];
+    __shared__ uint8_t turn[PART == kColMaxima ? 1 : RUNS][kColBlock * kColPitch];
     lds_int *tab_run = (lds_int *)table, *tab_row = (lds_int *)table + kMaxGroups + 1;
-    build_group_table<kTokenRun>(grp, 0, 1, tab_run, tab_row);
     const int col_blocks = (cols + kColBlock - 1) / kColBlock;
-    const int g = (int)(blockIdx.x / (unsigned)col_blocks);
+    int g = (int)(blockIdx.x / (unsigned)col_blocks), batch0 = 0;
+    if constexpr (PART != kColWhole) {
+        // (a group without rows gets no batch here: its scales of 1 are written below)
+        const int total = build_group_table<ROWS>(grp, 0, 1, (lds_int *)batch_table, tab_row);
+        if (g < total) {
+            const int batch = g;
+            g = group_of_tile(grp.groups, (lds_int *)batch_table, batch);
+            batch0 = batch - __builtin_amdgcn_readfirstlane(batch_table[g]);
+        } else {
+            // the last workgroups: what lies behind the last group, and the groups without rows
+            if (PART == kColMaxima || g < (int)(gridDim.x / (unsigned)col_blocks) - 1) return;
+            g = grp.groups;
+        }
+        __syncthreads();
+    }
+    build_group_table<kTokenRun>(grp, 0, 1, tab_run, tab_row);
     const int c0 = (int)(blockIdx.x % (unsigned)col_blocks) * kColBlock;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int cc = threadIdx.x & 7, slot = threadIdx.x >> 3;       // eight columns, four of the rows
@@ -272,14 +299,23 @@ __global__ __launch_bounds__(kColThreads) void quantize_columns_kernel(GroupSpec
         // behind the last group: zeros
         for (size_t at = ((size_t)tab_run[g] + wrun) * kTokenRun; at < ld; at += AT_ONCE * kTokenRun)
             if (c0 + wcol < cols) *reinterpret_cast<v4i *>(codes_t + (size_t)(c0 + wcol) * ld + at + wpiece * 16) = v4i{0, 0, 0, 0};
+        if (PART == kColCodes)
+            for (int e = threadIdx.x / kColBlock; e < grp.groups; e += kColThreads / kColBlock) {
+                const int col = c0 + threadIdx.x % kColBlock;
+                if (tab_row[e + 1] <= tab_row[e] && col < cols) scales[(size_t)e * cols + col] = 1.0f;
+            }
         return;
     }
-    const int first = tab_row[g], end = tab_row[g + 1];
+    // the rows of this workgroup: all of the group's, or those of one batch
+    const int first = tab_row[g] + batch0 * ROWS, group_end = tab_row[g + 1];
+    const int end = PART == kColWhole || group_end < first + ROWS ? group_end : first + ROWS;
     const int batches = end > first ? (end - first + ROWS - 1) / ROWS : 0;
+    const bool tail = c0 + kColBlock > cols && cols % 8 != 0;      // a thread's eight columns may end behind the last one
     QuantRaw raw[QUADS][4];
     auto load = [&](int batch) __attribute__((always_inline)) {
 #pragma unroll
         for (int q = 0; q < QUADS; ++q) {
+            if (first + batch * ROWS + q * (kColThreads / 2) >= end) continue;       // (uniform)
             const int r0 = first + batch * ROWS + q * (kColThreads / 2) + slot * 4;
             long src[4];
 #pragma unroll
@@ -287,8 +323,12 @@ __global__ __launch_bounds__(kColThreads) void quantize_columns_kernel(GroupSpec
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 raw[q][u] = QuantRaw{{0, 0, 0, 0}, {0, 0, 0, 0}};
-                if (src[u] >= 0 && src[u] < x_rows) raw[q][u] = quant_load_cols<TYPE, VEC>(x, (size_t)src[u] * x_stride, c, cols);
+                if (src[u] >= 0 && src[u] < x_rows && c + 8 <= cols) raw[q][u] = quant_load8_raw<TYPE>(x, (size_t)src[u] * x_stride + c);
             }
+            if (tail)
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (src[u] >= 0 && src[u] < x_rows && c < cols && c + 8 > cols) raw[q][u] = quant_load_some<TYPE>(x, (size_t)src[u] * x_stride + c, cols - c);
         }
     };
     // ---- the columns' largest magnitudes
@@ -297,7 +337,8 @@ __global__ __launch_bounds__(kColThreads) void quantize_columns_kernel(GroupSpec
     for (int b = 0; b < batches; ++b) {
         load(b);
 #pragma unroll
-        for (int q = 0; q < QUADS; ++q)
+        for (int q = 0; q < QUADS; ++q) {
+            if (first + b * ROWS + q * (kColThreads / 2) >= end) continue;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 float v[8];
@@ -305,29 +346,53 @@ __global__ __launch_bounds__(kColThreads) void quantize_columns_kernel(GroupSpec
 #pragma unroll
                 for (int i = 0; i < 8; ++i) odd |= quant_fold(v[i], amax[i]);
             }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-#pragma unroll
-        for (int off = 8; off < 64; off <<= 1) {
-            const uint32_t o = (uint32_t)__shfl_xor((int)amax[i], off, 64);
-            amax[i] = o > amax[i] ? o : amax[i];
         }
-        if (lane < 8) amax_of[wave][cc * 8 + i] = amax[i];
+    }
+    if constexpr (PART != kColCodes) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+            for (int off = 8; off < 64; off <<= 1) {
+                const uint32_t o = (uint32_t)__shfl_xor((int)amax[i], off, 64);
+                amax[i] = o > amax[i] ? o : amax[i];
+            }
+            if (lane < 8) amax_of[wave][cc * 8 + i] = amax[i];
+        }
     }
     const bool rough = __syncthreads_or(odd) != 0;
+    if constexpr (PART == kColMaxima) {
+        if (threadIdx.x < kColBlock && c0 + (int)threadIdx.x < cols) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                const uint32_t o = amax_of[w][threadIdx.x];
+                m = o > m ? o : m;
+            }
+            if (m != 0) atomicMax(reinterpret_cast<int *>(scales) + (size_t)g * cols + c0 + threadIdx.x, quant_scale_exponent<FMT>(m) << 23);
+        }
+        return;
+    }
     float inv[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        uint32_t m = 0;
+        int e = 127;
+        if constexpr (PART == kColCodes) {
+            // (0: no number but zeros.  The first batch writes the scale of 1 that stands for it, which reads as the same.)
+            if (c + i < cols) {
+                const int bits = __builtin_nontemporal_load(reinterpret_cast<const int *>(scales) + (size_t)g * cols + c + i);
+                e = bits == 0 ? 127 : bits >> 23;
+            }
+        } else {
+            uint32_t m = 0;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            const uint32_t o = amax_of[w][cc * 8 + i];
-            m = o > m ? o : m;
+            for (int w = 0; w < WAVES; ++w) {
+                const uint32_t o = amax_of[w][cc * 8 + i];
+                m = o > m ? o : m;
+            }
+            e = quant_scale_exponent<FMT>(m);
         }
-        const int e = quant_scale_exponent<FMT>(m);
         inv[i] = quant_inverse(e);
-        if (slot == 0 && c + i < cols) scales[(size_t)g * cols + c + i] = quant_scale(e);
+        if (batch0 == 0 && slot == 0 && c + i < cols) scales[(size_t)g * cols + c + i] = quant_scale(e);
     }
     // ---- the codes
     for (int b = batches - 1; b >= 0; --b) {
@@ -335,6 +400,7 @@ __global__ __launch_bounds__(kColThreads) void quantize_columns_kernel(GroupSpec
         __syncthreads();                                  // (the runs before have been written out)
 #pragma unroll
         for (int q = 0; q < QUADS; ++q) {
+            if (first + b * ROWS + q * (kColThreads / 2) >= end) continue;
             float v[4][8];
 #pragma unroll
             for (int u = 0; u < 4; ++u) quant_unpack8<TYPE>(raw[q][u], v[u]);
@@ -349,7 +415,7 @@ __global__ __launch_bounds__(kColThreads) void quantize_columns_kernel(GroupSpec
             const int r = b * RUNS + run;                 // run of the group
             if (first + r * kTokenRun >= end || c0 + wcol >= cols) continue;
             const uint32_t *p = reinterpret_cast<const uint32_t *>(turn[run] + wcol * kColPitch + wpiece * 16);
-            *reinterpret_cast<v4i *>(codes_t + (size_t)(c0 + wcol) * ld + ((size_t)tab_run[g] + r) * kTokenRun + wpiece * 16) = v4i{(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
+            *reinterpret_cast<v4i *>(codes_t + (size_t)(c0 + wcol) * ld + ((size_t)tab_run[g] + batch0 * RUNS + r) * kTokenRun + wpiece * 16) = v4i{(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
         }
     }
 }

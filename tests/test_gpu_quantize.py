@@ -210,6 +210,41 @@ def test_long_experts(pkg):
         check_columns(pkg, wide(gen, 3000, 136, dtype), [1, 2500, 0, 499], 1)
 
 
+@pytest.mark.parametrize("dtype", WIDE)
+@pytest.mark.parametrize("counts,cols", [([5000], 200), ([3000, 0, 1, 4100], 75), ([0, 0, 2600], 513), ([1025], 1)])
+def test_few_experts_with_many_rows(pkg, dtype, counts, cols):
+    """The walks split over the rows: infinities, NaNs and largest numbers in one part, columns of zeros, subnormals alone."""
+    gen = generator("split", cols)
+    rows = sum(counts)
+    x = wide(gen, rows, cols, dtype)
+    x[rows // 3, 0], x[rows - 1, cols // 2] = float("inf"), float("nan")
+    if cols > 3:
+        x[:, 1] = 0
+        x[:, 2] = torch.finfo(dtype).tiny / 2
+        x[rows // 2, 3] = torch.finfo(dtype).max
+    for fmt in (0, 1):
+        check_columns(pkg, x, counts, fmt)
+
+
+@pytest.mark.parametrize("dtype", WIDE)
+@pytest.mark.parametrize("shift,cols", [(1, 64), (3, 61), (1, 1000), (5, 4097), (1, 9000)])
+def test_any_place_and_length(pkg, dtype, shift, cols):
+    """Rows that start anywhere and are not whole pieces, what surrounds them stays out; codes that start anywhere."""
+    gen = generator("place", shift, cols)
+    rows = 37
+    store = torch.full((rows * (cols + 2) + 16,), float("inf"), dtype=dtype, device="cuda")
+    x = store[shift:shift + rows * (cols + 2)].view(rows, cols + 2)[:, :cols]
+    x.copy_(wide(gen, rows, cols, dtype))
+    v, s = quantized(x, 0, 1)
+    room = torch.full((rows * cols + 16,), 0x55, dtype=torch.uint8, device="cuda")
+    out = room[shift:shift + rows * cols].view(F8[0]).view(rows, cols)
+    got, scales = pkg.quantize_rows(x, 0, codes=out)
+    assert torch.equal(scales.double(), s)
+    same(got, v)
+    assert (room[:shift] == 0x55).all() and (room[shift + rows * cols:] == 0x55).all()
+    check_columns(pkg, x, [20, 0, 17], 0)
+
+
 def test_calls_captured_and_replayed(pkg):
     gen = generator("graph")
     x = wide(gen, 256, 512, torch.bfloat16)
