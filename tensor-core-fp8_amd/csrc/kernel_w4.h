@@ -589,28 +589,32 @@ __global__ __launch_bounds__(64 * kW4Waves, 4) void gemv_w4_kernel(W4Args p)
 }
 
 // The same for more rows of x than one block of 16 (16 * MT at a time), where x no longer fits LDS and the waves would wait for
-// it: K goes by in pieces of kW4PieceK, x through two LDS buffers and two sets of registers (a piece is read three pieces ahead), the
+// it: K goes by in pieces, x through two LDS buffers and two sets of registers (a piece is read three pieces ahead), the
 // weights straight into registers four pieces ahead, the scales staged for as many pieces as fit.  A wave takes TN blocks of
-// 16 columns, so that a read of x from LDS feeds TN products: with one the LDS is what bounds 64 rows.  Two waves along K.
+// 16 columns, so that a read of x from LDS feeds TN products: with one the LDS is what bounds 64 rows.  Two waves along K, or four
+// where the columns are few.
 //
 // Where the four lanes of a row have to share 32 consecutive weights (see above) their 16-byte loads are turned around by
 // swaps between lanes.  64 rows, integers in runs of 128: 4096 x 4096 21.5 us (the kernel above, in blocks of 64 rows, 69),
 // 17536 x 6784 with 58 rows 55 (100): the matrix unit, LDS and the vector unit take 0.4 to 0.8 us of a piece's 1.7 each, and two
 // waves on a SIMD in step overlap little of it.  Reading x a step ahead, or starting every workgroup at another piece, gains
 // nothing.
-constexpr int kW4PieceK = 256, kW4WideWk = 2, kW4WideWc = kW4Waves / kW4WideWk, kW4Ahead = 4;
-constexpr int kW4WideXPitch = kW4PieceK * 2 + 16;
-__host__ __device__ constexpr int w4_wide_x_bytes(int mt) { return 2 * 16 * mt * kW4WideXPitch; }
+constexpr int kW4Ahead = 4;
+// WK waves along K: a piece has 128 k of each, a workgroup 16 * TN columns of the others side by side
+__host__ __device__ constexpr int w4_piece(int wk) { return 128 * wk; }
+__host__ __device__ constexpr int w4_wide_cols(int wk, int tn) { return 16 * tn * (kW4Waves / wk); }
+__host__ __device__ constexpr int w4_wide_x_bytes(int mt, int wk) { return 2 * 16 * mt * w4_x_pitch(w4_piece(wk)); }
 
-template <bool F16, int MODE, int RUN, int MT, int KIND, int TN, bool CODES>
+template <bool F16, int MODE, int RUN, int MT, int KIND, int WK, int TN, bool CODES>
 __global__ __launch_bounds__(64 * kW4Waves) void gemm_w4_wide_kernel(W4Args p, int scale_pieces)
 {
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     constexpr bool PER_LANE = RUN == 128 || MODE == kW4Fp4Scaled;
-    constexpr int EB = w4_entry_bytes(MODE, KIND), COLS = 16 * TN * kW4WideWc, UNITS = kW4PieceK / 8;
-    static_assert(16 * MT * UNITS == MT * 64 * kW4Waves, "a thread stages MT pieces of eight numbers");
+    constexpr int EB = w4_entry_bytes(MODE, KIND), WC = kW4Waves / WK, COLS = w4_wide_cols(WK, TN), PIECE = w4_piece(WK), PITCH = w4_x_pitch(PIECE);
+    constexpr int UNITS = PIECE / 8, X_ROWS = 64 * kW4Waves / UNITS, XT = 16 * MT / X_ROWS;      // a thread stages every X_ROWS-th row's eight numbers
+    static_assert(XT * X_ROWS == 16 * MT && kW4Ahead % 2 == 0, "whole turns");
     const int lane = threadIdx.x & 63, fi = lane & 15, fq = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wc = wave % kW4WideWc, wk = wave / kW4WideWc;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wc = wave % WC, wk = wave / WC;
     const int g = blockIdx.y, n0 = blockIdx.x * COLS;
     int first, end;
     w4_group_rows(p, g, first, end);
@@ -621,26 +625,26 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemm_w4_wide_kernel(W4Args p, i
     const __amdgpu_buffer_rsrc_t rw = w4_rsrc(p.w + ((size_t)g * p.n + n0) * row_bytes, (size_t)(p.n - n0 < COLS ? p.n - n0 : COLS) * row_bytes);
     uint32_t w_at[TN];
 #pragma unroll
-    for (int c = 0; c < TN; ++c) w_at[c] = (uint32_t)(16 * (TN * wc + c) + fi) * (uint32_t)row_bytes + (uint32_t)(wk * (kW4PieceK / kW4WideWk / 2) + fq * 16);
-    const int pieces = (p.k + kW4PieceK - 1) / kW4PieceK;
+    for (int c = 0; c < TN; ++c) w_at[c] = (uint32_t)(16 * (TN * wc + c) + fi) * (uint32_t)row_bytes + (uint32_t)(wk * 64 + fq * 16);
+    const int pieces = (p.k + PIECE - 1) / PIECE;
     constexpr uint32_t elem = CODES ? 1 : 2;
-    LDS_AS uint8_t *xs = (LDS_AS uint8_t *)lds, *ss = xs + w4_wide_x_bytes(MT);
+    LDS_AS uint8_t *xs = (LDS_AS uint8_t *)lds, *ss = xs + w4_wide_x_bytes(MT, WK);
     const int x_unit = threadIdx.x % UNITS, x_first = threadIdx.x / UNITS;       // this thread's eight columns and first row of a piece
-    const int runs = scale_pieces * (kW4PieceK / RUN), s_pitch = w4_scale_pitch(runs, EB);
+    const int runs = scale_pieces * (PIECE / RUN), s_pitch = w4_scale_pitch(runs, EB);
     const LDS_AS uint8_t *s_lane[TN];
 #pragma unroll
-    for (int c = 0; c < TN; ++c) s_lane[c] = ss + (16 * (TN * wc + c) + fi) * s_pitch + (wk * (kW4PieceK / kW4WideWk / RUN) + (MODE == kW4Fp4Scaled && RUN == 32 ? fq : 0)) * EB;
-    const LDS_AS uint8_t *x_lane = xs + fi * kW4WideXPitch + wk * kW4PieceK + (PER_LANE ? 4 * fq : fq) * 16;
+    for (int c = 0; c < TN; ++c) s_lane[c] = ss + (16 * (TN * wc + c) + fi) * s_pitch + (wk * (128 / RUN) + (MODE == kW4Fp4Scaled && RUN == 32 ? fq : 0)) * EB;
+    const LDS_AS uint8_t *x_lane = xs + fi * PITCH + wk * 256 + (PER_LANE ? 4 * fq : fq) * 16;
 
     for (int m0 = first; m0 < end; m0 += 16 * MT) {
         const int rows = end - m0 < 16 * MT ? end - m0 : 16 * MT;
         const __amdgpu_buffer_rsrc_t rx = w4_rsrc(static_cast<const uint8_t *>(p.x) + (size_t)m0 * p.k * elem, (size_t)rows * p.k * elem);
-        v4i x_raw[2][MT], w_raw[kW4Ahead][TN];
-        auto load_x = [&](v4i (&r)[MT], int piece) __attribute__((always_inline)) {
-            const int k = piece * kW4PieceK + x_unit * 8;
+        v4i x_raw[2][XT], w_raw[kW4Ahead][TN];
+        auto load_x = [&](v4i (&r)[XT], int piece) __attribute__((always_inline)) {
+            const int k = piece * PIECE + x_unit * 8;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const uint32_t at = k < p.k ? ((uint32_t)(16 * i + x_first) * (uint32_t)p.k + (uint32_t)k) * elem : 0xFFFFFFF0u;
+            for (int i = 0; i < XT; ++i) {
+                const uint32_t at = k < p.k ? ((uint32_t)(X_ROWS * i + x_first) * (uint32_t)p.k + (uint32_t)k) * elem : 0xFFFFFFF0u;
                 if constexpr (CODES) {
                     const v2u c = __builtin_amdgcn_raw_buffer_load_b64(rx, (int)at, 0, 0);
                     r[i] = v4i{(int)c[0], (int)c[1], 0, 0};
@@ -649,16 +653,16 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemm_w4_wide_kernel(W4Args p, i
                 }
             }
         };
-        auto store_x = [&](const v4i (&r)[MT], int buffer) __attribute__((always_inline)) {
-            LDS_AS uint8_t *to = xs + buffer * (16 * MT * kW4WideXPitch) + x_first * kW4WideXPitch + x_unit * 16;
+        auto store_x = [&](const v4i (&r)[XT], int buffer) __attribute__((always_inline)) {
+            LDS_AS uint8_t *to = xs + buffer * (16 * MT * PITCH) + x_first * PITCH + x_unit * 16;
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-                *reinterpret_cast<LDS_AS v4i *>(to + 16 * i * kW4WideXPitch) = w4_order<MODE>(CODES ? w4_widen(v2u{(uint32_t)r[i][0], (uint32_t)r[i][1]}, p.x_type) : r[i]);
+            for (int i = 0; i < XT; ++i)
+                *reinterpret_cast<LDS_AS v4i *>(to + X_ROWS * i * PITCH) = w4_order<MODE>(CODES ? w4_widen(v2u{(uint32_t)r[i][0], (uint32_t)r[i][1]}, p.x_type) : r[i]);
         };
         auto load_w = [&](v4i (&r)[TN], int piece) __attribute__((always_inline)) {
 #pragma unroll
             for (int c = 0; c < TN; ++c)
-                r[c] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, piece < pieces ? (int)(w_at[c] + (uint32_t)piece * (kW4PieceK / 2)) : -16, 0, 2));
+                r[c] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rw, piece < pieces ? (int)(w_at[c] + (uint32_t)piece * (PIECE / 2)) : -16, 0, 2));
         };
         v4f total[MT][TN];
 #pragma unroll
@@ -674,7 +678,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemm_w4_wide_kernel(W4Args p, i
         load_x(x_raw[1], 2);
         for (int s0 = 0; s0 < pieces; s0 += scale_pieces) {
             const int cols = p.n - n0 < COLS ? p.n - n0 : COLS;
-            w4_stage_scales_any<F16, MODE, RUN, KIND>(p, ((size_t)g * p.n + n0) * p.per_row, s0 * kW4PieceK, runs, cols, COLS, ss, threadIdx.x, 64 * kW4Waves);
+            w4_stage_scales_any<F16, MODE, RUN, KIND>(p, ((size_t)g * p.n + n0) * p.per_row, s0 * PIECE, runs, cols, COLS, ss, threadIdx.x, 64 * kW4Waves);
             wait_lgkmcnt0();
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier();
@@ -695,8 +699,8 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemm_w4_wide_kernel(W4Args p, i
                         if constexpr (!PER_LANE) w4_turn(w[c]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
-                    const LDS_AS uint8_t *x_at = x_lane + (u & 1) * (16 * MT * kW4WideXPitch);
-                    const int s_at = (q - s0) * (kW4PieceK / RUN) * EB;
+                    const LDS_AS uint8_t *x_at = x_lane + (u & 1) * (16 * MT * PITCH);
+                    const int s_at = (q - s0) * (PIECE / RUN) * EB;
                     v4f sum[MT][TN];
                     float s[TN];
                     v4i minus[TN];
@@ -711,7 +715,7 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemm_w4_wide_kernel(W4Args p, i
                         const bool open = RUN == 32 || d == 0;         // a new run of the staged scales begins
                         v4i a[MT];
 #pragma unroll
-                        for (int i = 0; i < MT; ++i) a[i] = *reinterpret_cast<const LDS_AS v4i *>(x_at + 16 * i * kW4WideXPitch + (PER_LANE ? d : 4 * d) * 16);
+                        for (int i = 0; i < MT; ++i) a[i] = *reinterpret_cast<const LDS_AS v4i *>(x_at + 16 * i * PITCH + (PER_LANE ? d : 4 * d) * 16);
 #pragma unroll
                         for (int c = 0; c < TN; ++c) {
                             if constexpr (MODE != kW4Fp4Scaled)
@@ -751,13 +755,14 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemm_w4_wide_kernel(W4Args p, i
                 }
             }
         }
-        // ---- the two waves along K; register r of lane (fi, fq) holds y[16 i + 4 fq + r][column fi]
-        LDS_AS float *part = (LDS_AS float *)xs + wc * (TN * MT * 256);
-        if (wk == 1) {
+        // ---- the waves along K, in order; register r of lane (fi, fq) holds y[16 i + 4 fq + r][column fi]
+        static_assert((WK - 1) * WC * TN * MT * 1024 <= w4_wide_x_bytes(MT, WK), "no room for the partial sums");
+        LDS_AS float *part = (LDS_AS float *)xs + lane * 4;
+        if (wk > 0) {
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int c = 0; c < TN; ++c) *reinterpret_cast<LDS_AS v4f *>(part + ((i * TN + c) * 64 + lane) * 4) = total[i][c];
+                for (int c = 0; c < TN; ++c) *reinterpret_cast<LDS_AS v4f *>(part + ((((wk - 1) * WC + wc) * MT + i) * TN + c) * 256) = total[i][c];
         }
         __syncthreads();
         if (wk == 0) {
@@ -765,13 +770,15 @@ __global__ __launch_bounds__(64 * kW4Waves) void gemm_w4_wide_kernel(W4Args p, i
             for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int c = 0; c < TN; ++c) {
-                    const v4f other = *reinterpret_cast<const LDS_AS v4f *>(part + ((i * TN + c) * 64 + lane) * 4);
+                    v4f y = total[i][c];
+#pragma unroll
+                    for (int o = 0; o < WK - 1; ++o) y += *reinterpret_cast<const LDS_AS v4f *>(part + (((o * WC + wc) * MT + i) * TN + c) * 256);
                     const int col = n0 + 16 * (TN * wc + c) + fi;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int row = i * 16 + 4 * fq + r;
                         if (row < rows && col < p.n)
-                            store_out(p.y, (size_t)(m0 + row) * p.n + col, (total[i][c][r] + other[r]) * (p.x_scale ? p.x_scale[m0 + row] : 1.0f), p.y_type);
+                            store_out(p.y, (size_t)(m0 + row) * p.n + col, y[r] * (p.x_scale ? p.x_scale[m0 + row] : 1.0f), p.y_type);
                     }
                 }
         }

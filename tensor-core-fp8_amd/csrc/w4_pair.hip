@@ -2,6 +2,7 @@
 // times, with -DFP8GEMM_W4_F16=<0|1> (x and the expanded weights in bf16 or f16) -DFP8GEMM_W4_MODE=<kW4...> (w4_args.h).
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "dispatch.h"
 #include "kernel_w4.h"
@@ -74,39 +75,46 @@ hipError_t launch_w4_kernel(W4Args p, hipStream_t s)
     return hipGetLastError();
 }
 
-template <bool F16, int MODE, int RUN, int MT, int KIND, int TN, bool CODES>
+template <bool F16, int MODE, int RUN, int MT, int KIND, int WK, int TN, bool CODES>
 struct W4WideKernelTag {};
 
-template <bool F16, int MODE, int RUN, int MT, int KIND, int TN, bool CODES>
+template <bool F16, int MODE, int RUN, int MT, int KIND, int WK, int TN, bool CODES>
 hipError_t launch_w4_wide(const W4Args &p, hipStream_t s)
 {
-    constexpr int COLS = 16 * TN * kW4WideWc, EB = w4_entry_bytes(MODE, KIND), ROOM = kW4MaxLds - w4_wide_x_bytes(MT);
+    constexpr int COLS = w4_wide_cols(WK, TN), PIECE = w4_piece(WK), EB = w4_entry_bytes(MODE, KIND), ROOM = kW4MaxLds - w4_wide_x_bytes(MT, WK);
     // the scales of all of K, or of equal parts, whole turns of the weights' registers
-    const int pieces = (p.k + kW4PieceK - 1) / kW4PieceK;
-    auto bytes = [](int pieces_) { return COLS * w4_scale_pitch(pieces_ * (kW4PieceK / RUN), EB); };
-    static_assert(COLS * w4_scale_pitch(kW4Ahead * (kW4PieceK / RUN), EB) <= ROOM, "no room for the scales");
+    const int pieces = (p.k + PIECE - 1) / PIECE;
+    auto bytes = [](int pieces_) { return COLS * w4_scale_pitch(pieces_ * (PIECE / RUN), EB); };
+    static_assert(COLS * w4_scale_pitch(kW4Ahead * (PIECE / RUN), EB) <= ROOM, "no room for the scales");
     int parts = 1, scale_pieces;
     do {
         scale_pieces = ((pieces + parts - 1) / parts + kW4Ahead - 1) / kW4Ahead * kW4Ahead;
         ++parts;
     } while (bytes(scale_pieces) > ROOM);
-    auto kernel = gemm_w4_wide_kernel<F16, MODE, RUN, MT, KIND, TN, CODES>;
-    hipError_t e = allow_lds<W4WideKernelTag<F16, MODE, RUN, MT, KIND, TN, CODES>>(kernel, kW4MaxLds);
+    auto kernel = gemm_w4_wide_kernel<F16, MODE, RUN, MT, KIND, WK, TN, CODES>;
+    hipError_t e = allow_lds<W4WideKernelTag<F16, MODE, RUN, MT, KIND, WK, TN, CODES>>(kernel, kW4MaxLds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((p.n + COLS - 1) / COLS), (unsigned)p.groups), dim3(64 * kW4Waves), w4_wide_x_bytes(MT) + bytes(scale_pieces), s, p, scale_pieces);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((p.n + COLS - 1) / COLS), (unsigned)p.groups), dim3(64 * kW4Waves), w4_wide_x_bytes(MT, WK) + bytes(scale_pieces), s, p, scale_pieces);
     return hipGetLastError();
 }
 
 template <bool F16, int MODE, int RUN, int MT, int KIND>
 hipError_t launch_w4_tall(const W4Args &p, int busy, hipStream_t s)
 {
-    // Two blocks of 16 columns a wave where workgroups of 128 columns still keep half the CUs busy (us for one / two: 32 x
-    // 4096 x 4096 15.2 / 21.8, 64 x 4096 x 16384 22.3 / 28.2, 48 x 2048 x 24576 33.3 / 29.1, 17 x 8192 x 28672 49.0 / 40.7).
-    const bool wide = (long)(p.n + 127) / 128 * busy > 128;
+    // Workgroups of 128 columns (two blocks of 16 a wave) where they still keep half the CUs busy (us for 64 / 128 columns: 64 x 4096 x
+    // 16384 22.3 / 28.2, 32 x 4096 x 4096 15.2 / 21.8, 48 x 2048 x 24576 33.3 / 29.1, 17 x 8192 x 28672 49.0 / 40.7); else of 64; of 32
+    // with twice the waves along K where 64 keep less than half busy and K has several turns of its pieces (64 / 32: 20 x 4096 x
+    // 4096 14.8 / 11.5, 64 x 8192 x 2048 43 / 31, 30 x 2048 x 6000 10.7 / 9.6, but 40 x 1024 x 1024 9.6 / 11.2).
+    const long columns = (long)busy * p.n;
+    auto launch = [&](auto codes) {
+        constexpr bool CODES = decltype(codes)::value;
+        if (columns > 128 * 128) return launch_w4_wide<F16, MODE, RUN, MT, KIND, 2, 2, CODES>(p, s);
+        if (columns > 128 * 64 || p.k <= 1024) return launch_w4_wide<F16, MODE, RUN, MT, KIND, 2, 1, CODES>(p, s);
+        return launch_w4_wide<F16, MODE, RUN, MT, KIND, 4, 1, CODES>(p, s);
+    };
     if constexpr (F16)
-        if (p.x_type != FP8GEMM_T_F16)
-            return wide ? launch_w4_wide<F16, MODE, RUN, MT, KIND, 2, true>(p, s) : launch_w4_wide<F16, MODE, RUN, MT, KIND, 1, true>(p, s);
-    return wide ? launch_w4_wide<F16, MODE, RUN, MT, KIND, 2, false>(p, s) : launch_w4_wide<F16, MODE, RUN, MT, KIND, 1, false>(p, s);
+        if (p.x_type != FP8GEMM_T_F16) return launch(std::true_type{});
+    return launch(std::false_type{});
 }
 
 template <bool F16, int MODE, int RUN, int KIND>

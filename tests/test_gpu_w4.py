@@ -85,9 +85,10 @@ def test_lengths(pkg, k, n, m):
 @pytest.mark.parametrize("m", [20, 50])
 @pytest.mark.parametrize("run", [32, 128])
 def test_types_with_many_rows(pkg, w_fmt, scale, x_type, m, run):
-    """The kernel for more rows of x, one and two blocks of columns a wave (which one: n)."""
+    """The kernel for more rows of x, one and two blocks of columns a wave, two and four waves along K (which: n and k)."""
     run_case(pkg, m, 768, 40, run, w_fmt, scale, w_fmt == 0, x_type, torch.float32, "many")
     run_case(pkg, m, 384, 16900, run, w_fmt, scale, w_fmt == 0, x_type, torch.bfloat16, "many")
+    run_case(pkg, m, 1920, 70, run, w_fmt, scale, w_fmt == 0, x_type, torch.float32, "many")
 
 
 @pytest.mark.parametrize("k", [32, 64, 256, 288, 1056, 2048, 8192, 28672])
