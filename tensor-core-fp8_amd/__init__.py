@@ -495,9 +495,10 @@ def _ints(t, what):
 
 
 def _offsets(t):
-    if t.dim() != 1 or t.shape[0] < 2:
+    groups = t.numel() - 1
+    if groups < 1 or t.dim() != 1:
         raise Fp8GemmError("row_offsets holds one more element than there are experts")
-    return _ints(t, "row_offsets"), t.shape[0] - 1
+    return _ints(t, "row_offsets"), groups
 
 
 def _output(out, shape, dtype, like, stream):
@@ -524,10 +525,14 @@ def grouped_ld(rows, groups):
 
 def _wide_matrix(x, row_index):
     """rows of the result, columns, type code, row stride of a matrix to be quantised."""
-    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+    if x.dim() != 2:
         raise Fp8GemmError("x must be a matrix whose rows are contiguous")
     x_rows, cols = x.shape
-    stride = x.stride(0) if x_rows > 1 else cols
+    stride, step = x.stride()
+    if step != 1 and cols > 1:
+        raise Fp8GemmError("x must be a matrix whose rows are contiguous")
+    if x_rows <= 1:
+        stride = cols
     if stride < cols:
         raise Fp8GemmError("the rows of x overlap")
     return (x_rows if row_index is None else row_index.numel()), x_rows, cols, _wide_code(x.dtype), stride
@@ -543,7 +548,7 @@ def quantize_rows(x, fmt=E4M3, row_index=None, codes=None, scales=None, stream=N
     """(codes, scales) of the rows of x (float32 / bfloat16 / float16, unit column stride), or of the rows
     row_index (int32) names (an index outside x: a row of zeros): codes (rows, cols) float8, scales (rows,)
     float32 powers of two, x ~ codes * scales[:, None].  Through fp8gemm_quantize_rows."""
-    L = _setup() if _torch is None else lib()
+    L = _lib if _torch is not None and _lib is not None else _setup()
     rows, x_rows, cols, x_type, stride = _wide_matrix(x, row_index)
     device = _device_of(x, row_index, codes, scales)
     codes = _output(codes, (rows, cols), _fp8_dtype(fmt), x, stream)
@@ -559,7 +564,7 @@ def quantize_columns(x, row_offsets, fmt=E4M3, row_index=None, codes=None, scale
     """(codes, scales) of x transposed, for gemm_grouped_wgrad: codes (cols, grouped_ld(rows, groups)) float8,
     every expert's tokens in whole runs of 128 columns with zeros behind them, scales (groups, cols).
     row_index as in quantize_rows.  Through fp8gemm_quantize_columns."""
-    L = _setup() if _torch is None else lib()
+    L = _lib if _torch is not None and _lib is not None else _setup()
     rows, x_rows, cols, x_type, stride = _wide_matrix(x, row_index)
     device = _device_of(x, row_offsets, row_index, codes, scales)
     offs, groups = _offsets(row_offsets)
@@ -579,16 +584,19 @@ def gemm_grouped(a, b, row_offsets, a_scale=None, b_scale=None, out_dtype=None, 
     """out[i] = a_scale[i] * b_scale[g] * (a[i] . b[g]^T) for the rows i of every expert g: a (m, k), b (groups, n, k)
     codes, row_offsets (groups + 1,) int32, a_scale (m,), b_scale (groups, n) or (groups,) float32 or None.
     Rows outside the experts are left as they are (uninitialised when out is None).  Through fp8gemm_grouped."""
-    L = _setup() if _torch is None else lib()
+    L = _lib if _torch is not None and _lib is not None else _setup()
     device = _device_of(a, b, row_offsets, a_scale, b_scale, out)
-    if a.dim() != 2 or b.dim() != 3 or a.shape[1] != b.shape[2]:
-        raise Fp8GemmError("a (m, k) and b (groups, n, k) do not fit")
+    if a.dim() != 2 or b.dim() != 3:
+        raise Fp8GemmError("expected a (m, k) and b (groups, n, k)")
+    m, k = a.shape
+    matrices, n, b_k = b.shape
+    if b_k != k:
+        raise Fp8GemmError("inner dimensions differ: %d vs %d" % (k, b_k))
     if not (a.is_contiguous() and b.is_contiguous()):
         raise Fp8GemmError("operands must be contiguous")
     offs, groups = _offsets(row_offsets)
-    if b.shape[0] != groups:
-        raise Fp8GemmError("row_offsets is for %d experts, b holds %d" % (groups, b.shape[0]))
-    (m, k), n = a.shape, b.shape[1]
+    if matrices != groups:
+        raise Fp8GemmError("row_offsets is for %d experts, b holds %d" % (groups, matrices))
     out = _output(out, (m, n), out_dtype, a, stream)
     if m == 0:
         return out
@@ -604,16 +612,19 @@ def gemm_grouped_wgrad(a_t, b_t, row_offsets, rows, a_scale=None, b_scale=None, 
     """out[g] = a_scale[g][:, None] * b_scale[g] * (a_t . b_t^T over the tokens of expert g): a_t (m, ld), b_t (n, ld) codes
     as quantize_columns lays them out for `rows` rows, a_scale (groups, m), b_scale (groups, n) float32 or None;
     out (groups, m, n), added to what it holds if accumulate.  Through fp8gemm_grouped_wgrad."""
-    L = _setup() if _torch is None else lib()
+    L = _lib if _torch is not None and _lib is not None else _setup()
     device = _device_of(a_t, b_t, row_offsets, a_scale, b_scale, out)
-    if a_t.dim() != 2 or b_t.dim() != 2 or a_t.shape[1] != b_t.shape[1]:
-        raise Fp8GemmError("a_t (m, ld) and b_t (n, ld) do not fit")
+    if a_t.dim() != 2 or b_t.dim() != 2:
+        raise Fp8GemmError("expected a_t (m, ld) and b_t (n, ld)")
+    m, ld = a_t.shape
+    n, b_ld = b_t.shape
+    if b_ld != ld:
+        raise Fp8GemmError("a_t and b_t have rows of %d and %d columns" % (ld, b_ld))
     if not (a_t.is_contiguous() and b_t.is_contiguous()):
         raise Fp8GemmError("operands must be contiguous")
     if accumulate and out is None:
         raise Fp8GemmError("accumulate needs the tensor to add to")
     offs, groups = _offsets(row_offsets)
-    (m, ld), n = a_t.shape, b_t.shape[0]
     out = _output(out, (groups, m, n), out_dtype, a_t, stream)
     if rows == 0:
         if not accumulate:
@@ -631,23 +642,25 @@ def gemv_w4(x, w, scales, run, w_fmt=W4_INT, zeros=None, x_scale=None, row_offse
     low nibbles), scales (n, k/run) float32 / bfloat16 / float16 or uint8 (powers of two, 127 = 1), zeros (n, k/run)
     uint8 or None, x_scale (m,) float32 or None.  With row_offsets (groups + 1,) the rows of x are sorted by expert and
     w, scales, zeros have a leading axis of experts.  Through fp8gemm_gemv_w4 / fp8gemm_grouped_w4."""
-    L = _setup() if _torch is None else lib()
+    L = _lib if _torch is not None and _lib is not None else _setup()
     torch = _torch
     device = _device_of(x, w, scales, zeros, x_scale, row_offsets, out)
     if x.dim() != 2 or not (x.is_contiguous() and w.is_contiguous()):
         raise Fp8GemmError("x must be a matrix, operands contiguous")
     m, k = x.shape
+    wide = w.shape
     if row_offsets is None:
-        offs, groups, lead = None, 1, ()
+        offs, groups = None, 1
+        fits = len(wide) == 2
     else:
         offs, groups = _offsets(row_offsets)
-        lead = (groups,)
-    if w.dtype is not torch.uint8 or w.dim() != 2 + len(lead) or w.shape[:-2] != lead or 2 * w.shape[-1] != k:
+        fits = len(wide) == 3 and wide[0] == groups
+    if not fits or 2 * wide[-1] != k or w.dtype is not torch.uint8:
         raise Fp8GemmError("w must hold %d x n x k/2 bytes" % groups)
-    n = w.shape[-2]
+    n = wide[-2]
     if run <= 0 or k % run:
         raise Fp8GemmError("run must divide k")
-    shape = lead + (n, k // run)
+    shape = (n, k // run) if offs is None else (groups, n, k // run)
     if scales.shape != shape or not scales.is_contiguous():
         raise Fp8GemmError("scales must have the shape %s" % (shape,))
     if zeros is not None and (zeros.shape != shape or not zeros.is_contiguous() or zeros.dtype is not torch.uint8):

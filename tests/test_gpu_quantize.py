@@ -264,3 +264,24 @@ def test_calls_captured_and_replayed(pkg):
         vt, st = pkg.quantize_columns(x, off)
         assert torch.equal(v.view(torch.uint8), codes.view(torch.uint8)) and torch.equal(s, scales)
         assert torch.equal(vt.view(torch.uint8), codes_t.view(torch.uint8)) and torch.equal(st, scales_t)
+
+
+def test_split_columns_captured_and_replayed(pkg):
+    """Few experts with many rows, replayed with other numbers and another cut: scales sink as well as rise."""
+    gen = generator("split graph")
+    rows, cols = 4096, 130
+    x = wide(gen, rows, cols, torch.bfloat16)
+    off = offsets_of([4000, 96])
+    codes, scales = pkg.quantize_columns(x, off)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pkg.quantize_columns(x, off, codes=codes, scales=scales)
+    for turn, counts in enumerate(([4000, 96], [10, 4086], [4096, 0], [0, 1700])):
+        x.copy_(wide(gen, rows, cols, torch.bfloat16) * 2.0 ** (-3 * turn))
+        off.copy_(offsets_of(counts))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want, want_s = pkg.quantize_columns(x, off)
+        assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales, want_s)
+        check_columns(pkg, x, counts, 0)

@@ -288,3 +288,29 @@ def test_weights_beyond_32_bits(pkg):
         ref = x[r:r + 1].double() @ v.t().contiguous()
         bound = 62.0 * s[g, -2000:].double().repeat_interleave(run, -1)
         assert ((y[r:r + 1, -2000:].double() - ref).abs() <= tolerance(x[r:r + 1].double(), v, bound, torch.float32, ref)).all()
+
+
+def test_many_rows_captured_and_replayed(pkg):
+    gen = generator("many graph")
+    n, k, run = 200, 2304, 64
+    w, s, z = weights(gen, (3,), n, k, run, 0, torch.float16, True)
+    x = torch.randn((90, k), generator=gen, device="cuda").to(torch.bfloat16)
+    off = offsets_of([40, 0, 50])
+    y = torch.zeros((90, n), device="cuda")
+    pkg.gemv_w4(x, w, s, run, zeros=z, row_offsets=off, out=y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        pkg.gemv_w4(x, w, s, run, zeros=z, row_offsets=off, out=y)
+    for counts in ([40, 0, 50], [1, 88, 1], [0, 0, 90], [30, 30, 30]):
+        x.copy_(torch.randn((90, k), generator=gen, device="cuda"))
+        off.copy_(offsets_of(counts))
+        y.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, pkg.gemv_w4(x, w, s, run, zeros=z, row_offsets=off))
+        for g in range(3):
+            lo, hi = int(off[g]), int(off[g + 1])
+            if hi > lo:
+                ref = x[lo:hi].double() @ w4_values(w[g], s[g], run, 0, z[g]).t().contiguous()
+                bound = 62.0 * scale_values(s[g]).repeat_interleave(run, -1)
+                assert ((y[lo:hi].double() - ref).abs() <= tolerance(x[lo:hi].double(), None, bound, torch.float32, ref)).all()
