@@ -595,7 +595,7 @@ __global__ __launch_bounds__(64 * kW4Waves, 4) void gemv_w4_kernel(W4Args p)
 // where the columns are few.
 //
 // Where the four lanes of a row have to share 32 consecutive weights (see above) their 16-byte loads are turned around by
-// swaps between lanes.  64 rows, integers in runs of 128: 4096 x 4096 21.5 us (the kernel above, in blocks of 64 rows, 69),
+// swaps between lanes.  64 rows, integers in runs of 128: 4096 x 4096 18 us (the kernel above, in blocks of 64 rows, 69),
 // 17536 x 6784 with 58 rows 55 (100): the matrix unit, LDS and the vector unit take 0.4 to 0.8 us of a piece's 1.7 each, and two
 // waves on a SIMD in step overlap little of it.  Reading x a step ahead, or starting every workgroup at another piece, gains
 // nothing.
