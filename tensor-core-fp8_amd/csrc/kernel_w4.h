@@ -21,7 +21,7 @@
 // A workgroup of eight waves is WC waves side by side (16 columns each) times WK waves along K, whose sums are
 // added in wave order through LDS: few columns still fill the chip.  It goes through several blocks of columns;
 // x and the scales of all of them are staged in LDS once, then the waves' rings run without a break over all blocks.
-// One row, 28672 x 8192 integers in runs of 128: 27 us, 4.5 TB/s; runs of 32 43 us, where the vector unit is the bound.
+// One row, 28672 x 8192 integers in runs of 128: 27 us, 4.5 TB/s; runs of 32 38 us, where the vector unit is the bound.
 #ifndef FP8GEMM_KERNEL_W4_H
 #define FP8GEMM_KERNEL_W4_H
 

@@ -26,11 +26,13 @@ hipError_t launch_w4_kernel(W4Args p, hipStream_t s)
     const int rows = std::min((p.rows + busy - 1) / busy, 16);
     const long col_tiles = (p.n + 15) / 16, row_bytes = p.k / 2;
     // How the eight waves are laid out, how many workgroups share a CU and how many blocks of columns each takes: the
-    // least time in units of one ring stage of a workgroup -- half a unit to add the waves along K up, six to
-    // start a pass, more to stage many rows of x, and two workgroups on a CU hide 15 % of each other's time.  (Two only
-    // where the registers of 16 waves fit.  MI355X, one row, us for the pick / the best of the eight layouts: 28672 x 8192 integers
-    // in runs of 128 27.1 / 27.1, of 32 43.9 / 36.5; 8192 x 8192 13.4 / 11.9; 4096 x 4096 7.9 / 7.9; 16 rows 28672 x 8192 42.5 / 42.8.)
+    // least time in units of one ring stage of a workgroup -- one unit to add the waves along K up, one to start a pass, more to
+    // stage the rows of x or where not all of x fits, and two workgroups on a CU hide 28 % of each other's time.  The experts that
+    // will have rows are counted as if every row fell on any of them.  Fitted to 140 calls (integers in runs of 32 and 128, e2m1, 1 to
+    // 14 rows of one matrix, 8 to 40 of 8 and 32 experts): the pick takes 0.7 % longer than the best of the eight layouts on
+    // average, 12 % at worst.
     constexpr int EB = w4_entry_bytes(MODE, KIND);
+    const double active = p.groups > 1 ? p.groups * (1.0 - std::pow(1.0 - 1.0 / p.groups, p.rows)) : 1.0;
     double best = 1e30;
     int best_lds = 0;
     p.part_rows = std::min(p.rows, 16);
@@ -50,10 +52,10 @@ hipError_t launch_w4_kernel(W4Args p, hipStream_t s)
             // (K in pieces: a pass for every block and piece)
             const long at_once = fits ? std::min(each, (room - x_bytes) / block_bytes) : 1;
             const double passes = fits ? (double)((each + at_once - 1) / at_once) : (double)each * (x_bytes + block_bytes) / room;
-            const double stages = (double)((p.k + unit - 1) / unit), staging = (fits ? 1.0 : (double)each) * rows * whole / 7000.0;
-            const long groups_of_waves = (blocks + each - 1) / each * busy, on_a_cu = (groups_of_waves + 255) / 256;
-            const double cost = (double)on_a_cu * (each * (stages + (wk > 1 ? 0.5 : 0.0)) + staging) * (on_a_cu > 1 && per_cu > 1 ? 0.85 : 1.0) +
-                                (double)((on_a_cu + per_cu - 1) / per_cu) * passes * 6.0;
+            const double stages = (double)((p.k + unit - 1) / unit), staging = (fits ? 1.0 : (double)each) * rows * whole / 12500.0;
+            const double on_a_cu = std::ceil((double)((blocks + each - 1) / each) * active / 256.0);
+            const double cost = on_a_cu * (each * (stages + (wk > 1 ? 1.15 : 0.0)) + staging) * (on_a_cu > 1.0 && per_cu > 1 ? 0.72 : 1.0) +
+                                std::max(1.0, on_a_cu / per_cu) * passes * 1.25 + (fits ? 0.0 : 1.7);
             if (cost < best) {
                 best = cost;
                 p.wk_shift = wk == 1 ? 0 : (wk == 2 ? 1 : (wk == 4 ? 2 : 3));
