@@ -158,9 +158,16 @@ def check(code):
         raise Fp8GemmError("fp8gemm error %d: %s" % (code, lib().fp8gemm_error_string(code).decode()))
 
 
+def _sizes(*sizes):
+    """Refuses what does not fit the C entry points' ints (ctypes would keep the low 32 bits and say nothing)."""
+    if max(sizes) > 0x7FFFFFFF or min(sizes) < -0x7FFFFFFF:
+        raise Fp8GemmError("sizes go up to 2^31 - 1, got %s" % (sizes,))
+
+
 def plan(m, k, n, stages=2):
     """(family, variant, K slices, columns per wave | rotation mode) that the automatic
     selection uses for a shape."""
+    _sizes(m, k, n)
     out = (ctypes.c_int * 4)()
     check(lib().fp8gemm_plan(m, k, n, stages, out))
     return tuple(out)
@@ -238,6 +245,7 @@ def gemm(a, b, out=None, a_fmt=None, b_fmt=None, stages=2, algo=ALGO_AUTO, varia
     n, k2 = b.shape
     if k != k2:
         raise Fp8GemmError("inner dimensions differ: %d vs %d" % (k, k2))
+    _sizes(m, k, n)
     fa, fb = _fmt_of(a, a_fmt), _fmt_of(b, b_fmt)
     if out is None:
         out = torch.empty((m, n), dtype=torch.float32, device=a.device)
@@ -267,6 +275,7 @@ def gemm_ex(a, b, out_dtype=None, out=None, alpha=1.0, a_scale=None, b_scale=Non
     n, k2 = b.shape
     if k != k2:
         raise Fp8GemmError("inner dimensions differ: %d vs %d" % (k, k2))
+    _sizes(m, k, n)
     if out is None:
         out = torch.empty((m, n), dtype=out_dtype or torch.float32, device=a.device)
     code = {torch.float32: OUT_F32, torch.bfloat16: OUT_BF16, torch.float16: OUT_F16}[out.dtype]
@@ -293,6 +302,7 @@ def gemm_epilogue(a, b, out_dtype=None, out=None, alpha=1.0, beta=0.0, c=None, a
     n, k2 = b.shape
     if k != k2:
         raise Fp8GemmError("inner dimensions differ: %d vs %d" % (k, k2))
+    _sizes(m, k, n)
     codes = {torch.float32: OUT_F32, torch.bfloat16: OUT_BF16, torch.float16: OUT_F16}
     if out is None:
         out = torch.empty((m, n), dtype=out_dtype or torch.float32, device=a.device)
@@ -313,6 +323,7 @@ _PAIR = {(E4M3, E4M3): "e4m3_e4m3", (E5M2, E5M2): "e5m2_e5m2", (E4M3, E5M2): "e4
 
 
 def _entry(m, k, n, a, b, out, stage):
+    _sizes(m, k, n)
     fn = getattr(lib(), "fp8gemm_%s_stage%d" % (_PAIR[(_fmt_of(a, None), _fmt_of(b, None))], stage))
     return fn(m, k, n, a.data_ptr(), b.data_ptr(), out.data_ptr())
 
@@ -347,6 +358,7 @@ def spmm_bell(values, block_cols, block, b, k, s_fmt=None, b_fmt=None, out=None,
         raise Fp8GemmError("values / block_cols do not fit the block size")
     vector = b.dim() == 1
     n = 1 if vector else b.shape[0]
+    _sizes(m, k, n, block, ell_cols)
     if (b.shape[0] if vector else b.shape[1]) != k:
         raise Fp8GemmError("b does not have k columns")
     if out is None:
@@ -371,6 +383,7 @@ def spmm_csr(values, row_offsets, col_idx, b, k, s_fmt=None, b_fmt=None, out=Non
     m = row_offsets.numel() - 1
     vector = b.dim() == 1
     n = 1 if vector else b.shape[0]
+    _sizes(m, k, n)
     if (b.shape[0] if vector else b.shape[1]) != k:
         raise Fp8GemmError("b does not have k columns")
     if out is None:
@@ -405,6 +418,7 @@ def sddmm(row_offsets, col_idx, vec_length, lhs, rhs, l_fmt=None, r_fmt=None, ou
     k = lhs.shape[1]
     if lhs.shape[0] != m_vec * vec_length or rhs.shape[1] != k:
         raise Fp8GemmError("lhs / rhs do not fit the pattern")
+    _sizes(m_vec, k, vec_length)
     if out is None:
         out = torch.empty((col_idx.numel(), vec_length), dtype=torch.float32, device=lhs.device)
     check(lib().fp8gemm_sddmm(m_vec, k, vec_length, _dev_ints(row_offsets), _dev_ints(col_idx), lhs.data_ptr(), _fmt_of(lhs, l_fmt),
@@ -498,6 +512,7 @@ def _offsets(t):
     groups = t.numel() - 1
     if groups < 1 or t.dim() != 1:
         raise Fp8GemmError("row_offsets holds one more element than there are experts")
+    _sizes(groups)
     return _ints(t, "row_offsets"), groups
 
 
@@ -520,6 +535,7 @@ def _fill(t, value, stream):
 
 def grouped_ld(rows, groups):
     """Columns of a transposed operand of gemm_grouped_wgrad for `rows` rows in `groups` experts (0 for no rows)."""
+    _sizes(rows, groups)
     return lib().fp8gemm_grouped_ld(rows, groups)
 
 
@@ -535,7 +551,9 @@ def _wide_matrix(x, row_index):
         stride = cols
     if stride < cols:
         raise Fp8GemmError("the rows of x overlap")
-    return (x_rows if row_index is None else row_index.numel()), x_rows, cols, _wide_code(x.dtype), stride
+    rows = x_rows if row_index is None else row_index.numel()
+    _sizes(rows, x_rows, cols)
+    return rows, x_rows, cols, _wide_code(x.dtype), stride
 
 
 def _fp8_dtype(fmt):
@@ -592,6 +610,7 @@ def gemm_grouped(a, b, row_offsets, a_scale=None, b_scale=None, out_dtype=None, 
     matrices, n, b_k = b.shape
     if b_k != k:
         raise Fp8GemmError("inner dimensions differ: %d vs %d" % (k, b_k))
+    _sizes(m, k, n)
     if not (a.is_contiguous() and b.is_contiguous()):
         raise Fp8GemmError("operands must be contiguous")
     offs, groups = _offsets(row_offsets)
@@ -620,6 +639,7 @@ def gemm_grouped_wgrad(a_t, b_t, row_offsets, rows, a_scale=None, b_scale=None, 
     n, b_ld = b_t.shape
     if b_ld != ld:
         raise Fp8GemmError("a_t and b_t have rows of %d and %d columns" % (ld, b_ld))
+    _sizes(rows, m, n, ld)
     if not (a_t.is_contiguous() and b_t.is_contiguous()):
         raise Fp8GemmError("operands must be contiguous")
     if accumulate and out is None:
@@ -658,6 +678,7 @@ def gemv_w4(x, w, scales, run, w_fmt=W4_INT, zeros=None, x_scale=None, row_offse
     if not fits or 2 * wide[-1] != k or w.dtype is not torch.uint8:
         raise Fp8GemmError("w must hold %d x n x k/2 bytes" % groups)
     n = wide[-2]
+    _sizes(m, k, n)
     if run <= 0 or k % run:
         raise Fp8GemmError("run must divide k")
     shape = (n, k // run) if offs is None else (groups, n, k // run)

@@ -99,3 +99,29 @@ def test_python_checks_need_no_gpu(pkg):
         pkg.quantize_columns(torch.zeros(4, 64), off)
     with pytest.raises(pkg.Fp8GemmError):
         pkg.gemv_w4(torch.zeros(1, 64, dtype=torch.bfloat16), torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2), 32)
+
+
+WRAPS = (1 << 32) + 256         # what is left of it in 32 bits is a size that every operator takes
+
+
+def test_sizes_that_an_int_cuts_off(pkg):
+    """A size beyond an int would reach the C entry points as its low 32 bits: refused before."""
+    import torch
+    for rows, groups in ((WRAPS, 1), (5, WRAPS), (1 << 31, 1), (-WRAPS, 1)):
+        with pytest.raises(pkg.Fp8GemmError):
+            pkg.grouped_ld(rows, groups)
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.plan(WRAPS, 256, 256)
+    off = torch.empty(WRAPS + 1, dtype=torch.int32, device="meta")
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg._offsets(off)
+    pkg._setup()
+    for shape, index in (((1, WRAPS), None), ((WRAPS, 1), None), ((4, 8), WRAPS), ((WRAPS, 1), 4)):
+        x = torch.empty(shape, dtype=torch.bfloat16, device="meta")
+        with pytest.raises(pkg.Fp8GemmError):
+            pkg._wide_matrix(x, None if index is None else torch.empty(index, dtype=torch.int32, device="meta"))
+    assert pkg._wide_matrix(torch.empty((1, 1 << 30), dtype=torch.bfloat16, device="meta"), None) == (1, 1, 1 << 30, pkg.OUT_BF16, 1 << 30)
+    # what the entry points do before any device is looked at
+    a = torch.empty((4, 64), dtype=torch.float8_e4m3fn, device="meta")
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.GEMM(4, 64, WRAPS, a, a, a)

@@ -189,3 +189,32 @@ def test_results_on_a_named_stream_are_its_memory(pkg):
         got, got_s = pkg.quantize_rows(x, stream=side)
         torch.cuda.synchronize()
         assert torch.equal(got.view(torch.uint8), want.view(torch.uint8)) and torch.equal(got_s, want_s)
+
+
+def test_sizes_that_an_int_cuts_off(pkg):
+    """Rows, columns and lengths of 2^32 and more are refused, not taken for what is left of them in 32 bits."""
+    wraps = (1 << 32) + 256
+    one = offsets_of([1])
+    flat = torch.empty((1, wraps), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.quantize_rows(flat)
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.quantize_columns(flat, one)
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.quantize_rows(flat.view(wraps, 1))
+    eight = flat.view(torch.float8_e4m3fn)[:, :wraps]
+    few = torch.zeros((1, 256), dtype=torch.float8_e4m3fn, device="cuda")
+    for a, b in ((eight, eight), (few[:, :1].contiguous(), eight.view(wraps, 1))):
+        with pytest.raises(pkg.Fp8GemmError):
+            pkg.gemm_grouped(a, b[None], one)
+        with pytest.raises(pkg.Fp8GemmError):
+            pkg.gemm(a, b)
+        with pytest.raises(pkg.Fp8GemmError):
+            pkg.gemm_ex(a, b)
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.gemm_grouped_wgrad(few, few, one, wraps)
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.gemm_grouped_wgrad(eight, eight, one, 1)
+    w = flat.view(torch.uint8)[:, :wraps // 2]
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.gemv_w4(flat, w, torch.empty((1, wraps // 256), device="cuda"), 256)
