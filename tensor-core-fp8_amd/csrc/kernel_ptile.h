@@ -550,6 +550,7 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
         const int m0 = GROUPED == kGroupedRows ? g_row0 : tile_m * BM, n0 = tile_n * BN;
         const int m_end = GROUPED == kGroupedRows ? g_row_end : M;
         const int c_group = g_id, c_set = g_set;       // (the planned item changes before the epilogue)
+        const bool c_none = GROUPED == kGroupedK && g_kt == 0;       // no tokens: zeros whatever the scales are, or C as it is
 
         // accumulators: TM x TN blocks of 32 x 32 (16 registers each), or twice as many
         // blocks of 16 x 16 each way (4 registers each); 256 registers per lane either way
@@ -857,6 +858,7 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
                     const LDS_AS float *sa = (const LDS_AS float *)(lds + S::PTILE_LDS_BYTES + kGroupTableOffset + c_set * (BM + BN) * 4);
                     const LDS_AS float *sb = sa + BM;
                     const bool quads = N % 4 == 0 && reinterpret_cast<uintptr_t>(C) % 16 == 0;
+                    const bool scaled_a = grp.a_scale && !c_none, scaled_b = grp.b_scale && !c_none;
                     v4f buf[NR], fb = {1.0f, 1.0f, 1.0f, 1.0f};
                     float fa[NR];
                     if (!quads || grp.accumulate) {
@@ -864,23 +866,23 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
 #pragma unroll 1
                         for (int r0 = 0; r0 < 32; r0 += RPI_ST) {
                             const v4f v = *reinterpret_cast<const v4f *>(stg + (r0 + rl) * ROWB + cl * 16);
-                            const float a = grp.a_scale ? sa[lrow0 + r0] : 1.0f;
+                            const float a = scaled_a ? sa[lrow0 + r0] : 1.0f;
                             const size_t index = first + (size_t)r0 * ldo;
-                            if (m0 + lrow0 + r0 < m_end)
+                            if (m0 + lrow0 + r0 < m_end && !(c_none && grp.accumulate))
                                 for (int e = 0; e < 4; ++e)
                                     if (n0 + lcol_ + e < N) {
-                                        const float y = v[e] * a * (grp.b_scale ? sb[lcol_ + e] : 1.0f);
+                                        const float y = v[e] * a * (scaled_b ? sb[lcol_ + e] : 1.0f);
                                         store_out(C, index + e, grp.accumulate ? y + load_in(C, index + e, grp.type) : y, grp.type);
                                     }
                         }
                         if constexpr (ST + 1 < NSTEP) stage_strip(std::integral_constant<int, ST + 1>{});
                         return;
                     }
-                    if (grp.b_scale) fb = *reinterpret_cast<const LDS_AS v4f *>(sb + lcol_);
+                    if (scaled_b) fb = *reinterpret_cast<const LDS_AS v4f *>(sb + lcol_);
 #pragma unroll
                     for (int u = 0; u < NR; ++u) {
                         buf[u] = *reinterpret_cast<const v4f *>(stg + (u * RPI_ST + rl) * ROWB + cl * 16);
-                        fa[u] = grp.a_scale ? sa[lrow0 + u * RPI_ST] : 1.0f;
+                        fa[u] = scaled_a ? sa[lrow0 + u * RPI_ST] : 1.0f;
                     }
                     if constexpr (ST + 1 < NSTEP) stage_strip(std::integral_constant<int, ST + 1>{});
                     __builtin_amdgcn_sched_barrier(0);

@@ -379,3 +379,35 @@ def test_wgrad_output_anywhere(pkg, dtype):
             pkg.gemm_grouped_wgrad(a, b, off, 130, out=out, variant=variant)
             check_wgrad(out, at, cs, a, b, None, None, dtype)
             assert (store[:shift] == 3.0).all() and (store[shift + size:] == 3.0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [256, 131])
+def test_wgrad_scales_of_experts_without_tokens(pkg, n, dtype):
+    """Scales that are no numbers, at experts that have no tokens: zeros, or what was there to its last bit."""
+    gen = generator("wgrad no tokens")
+    counts, m = [0, 200, 0, 0, 3, 0], 300
+    off, a, at, cs = transposed(gen, counts, m, 1)
+    _, b, _, _ = transposed(gen, counts, n, 0)
+    sa, sb = powers(gen, len(cs), m), powers(gen, len(cs), n)
+    odd = torch.tensor([float("nan"), float("inf"), -float("inf")], device="cuda")
+    for g, c in enumerate(cs):
+        if not c:
+            sa[g] = odd[torch.arange(m, device="cuda") % 3]
+            sb[g] = odd[(torch.arange(n, device="cuda") + g) % 3]
+    bits = torch.int32 if dtype == torch.float32 else torch.int16
+    held = torch.randn((len(cs), m, n), generator=gen, device="cuda").to(dtype)
+    held[:, ::7] = -0.0
+    held[:, 1::7] = float("inf")
+    held[:, 2::7] = float("nan")
+    for variant in WGRAD_VARIANTS:
+        for x, y in ((sa, sb), (sa, None), (None, sb)):
+            out = torch.full((len(cs), m, n), 5.0, dtype=dtype, device="cuda")
+            pkg.gemm_grouped_wgrad(a, b, off, sum(cs), a_scale=x, b_scale=y, out=out, variant=variant)
+            into = held.clone()
+            pkg.gemm_grouped_wgrad(a, b, off, sum(cs), a_scale=x, b_scale=y, out=into, accumulate=True, variant=variant)
+            for g, c in enumerate(cs):
+                if not c:
+                    assert not out[g].view(bits).any(), (variant, g)
+                    assert torch.equal(into[g].view(bits), held[g].view(bits)), (variant, g)
+            check_wgrad(out[[1, 4]], [at[1], at[4]], [cs[1], cs[4]], a, b, None if x is None else x[[1, 4]], None if y is None else y[[1, 4]], dtype)
