@@ -199,7 +199,11 @@ int fp8gemm_quantize_columns(int groups, int rows, int cols, const int *row_offs
  * n x (k / run) bytes of 0 .. 15 (the low four bits count), or NULL for 8 everywhere (FP8GEMM_W4_INT only).
  * run % 32 == 0, k % run == 0.  x: m x k of x_type (FP8GEMM_T_BF16, _F16, _E4M3, _E5M2), x_scale: m floats or NULL
  * for 1; y: m x n of y_type (FP8GEMM_OUT_*).  x and w 16-byte aligned.  Weights, scales and x enter unrounded, sums
- * are fp32.  (A row of x that holds an infinity gives NaN or infinities with FP8GEMM_W4_INT.)
+ * are fp32.  Ranges that this leaves, all of x in bf16: FP8GEMM_W4_INT sums up to 128 products of x with 16 + nibble and
+ * with 16 + zero before it applies the scale, so numbers of 2^116 and more may end as NaN or infinities where the formula
+ * is finite (as an infinity in x does, of any type); FP8GEMM_W4_E2M1 with _E8M0 scales multiplies bf16 numbers
+ * e2m1 * scale, of which those of 2^128 and more are infinities (byte 253 with 4 and 6, byte 254 with 2 to 6); with other
+ * scales it sums up to 128 products of x with e2m1 before it applies them, which stay finite for x below 2^118.
  * fp8gemm_grouped_w4: the rows sorted by expert as above, w, w_scales and w_zeros with `groups` matrices one
  * behind the other; only the experts that have rows are read.
  */

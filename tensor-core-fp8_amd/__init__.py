@@ -661,7 +661,8 @@ def gemv_w4(x, w, scales, run, w_fmt=W4_INT, zeros=None, x_scale=None, row_offse
     """y = x W^T for W in 4 bits: x (m, k) bfloat16 / float16 / fp8 codes, w (n, k/2) uint8 (even columns in the
     low nibbles), scales (n, k/run) float32 / bfloat16 / float16 or uint8 (powers of two, 127 = 1), zeros (n, k/run)
     uint8 or None, x_scale (m,) float32 or None.  With row_offsets (groups + 1,) the rows of x are sorted by expert and
-    w, scales, zeros have a leading axis of experts.  Through fp8gemm_gemv_w4 / fp8gemm_grouped_w4."""
+    w, scales, zeros have a leading axis of experts.  Through fp8gemm_gemv_w4 / fp8gemm_grouped_w4 (fp8gemm.h: how large
+    bfloat16 x and scale bytes may be)."""
     L = _lib if _torch is not None and _lib is not None else _setup()
     torch = _torch
     device = _device_of(x, w, scales, zeros, x_scale, row_offsets, out)

@@ -7,11 +7,12 @@
 // row of x the matrix unit does in 16 clocks what 512 multiply-adds would take, and the vector unit is left
 // to the expansion, one instruction per weight:
 //   integers: a nibble q is masked into the mantissa of 16.0, which makes 16 + q; a second MFMA on the same x
-//     with -(16 + zero) in place of W takes the excess out (all exact: small integers in 16 bits, sums in fp32),
-//     so zero points cost no instruction per weight (taking it out as (16 + zero) times the sum of the run's x
+//     with -(16 + zero) in place of W takes the excess out (exact factors: small integers in 16 bits; sums in fp32,
+//     so that x from 2^116 on, an infinity among them, can overflow both to a NaN),
+//     and zero points cost no instruction per weight (taking it out as (16 + zero) times the sum of the run's x
 //     saves those MFMAs and loses more at the staging of x, from four rows on by a factor);
 //   e2m1: the conversion instruction, two weights at a time, which also applies power-of-two scales where
-//     x is bf16 (exact: bf16 has fp32's exponents).
+//     x is bf16 (exact but for weights of 2^128 and more, byte 253 on: bf16 has fp32's exponents, down to 2^-133).
 // Other scales multiply the fp32 sum of a run, so neither weights nor scales are rounded.
 //
 // Which 8 of 32 consecutive k a lane holds is free as long as x agrees.  Runs of whole 128 k: a lane takes 32

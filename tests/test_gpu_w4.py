@@ -4,7 +4,7 @@ import zlib
 import pytest
 import torch
 
-from expert_util import F8, offsets_of, pow2, rounding, scale_values, w4_values
+from expert_util import E2M1, F8, offsets_of, pow2, rounding, scale_values, w4_values
 
 pytestmark = pytest.mark.gpu
 
@@ -314,3 +314,32 @@ def test_many_rows_captured_and_replayed(pkg):
                 ref = x[lo:hi].double() @ w4_values(w[g], s[g], run, 0, z[g]).t().contiguous()
                 bound = 62.0 * scale_values(s[g]).repeat_interleave(run, -1)
                 assert ((y[lo:hi].double() - ref).abs() <= tolerance(x[lo:hi].double(), None, bound, torch.float32, ref)).all()
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("x_type", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("w_fmt", [1, 0])
+def test_scale_bytes_with_every_weight(pkg, w_fmt, x_type, many):
+    """Every scale byte with every 4-bit weight and numbers of x from one end of the type to the other: one-hot rows, exact
+    wherever weight, scale and their product are numbers that the header speaks of."""
+    k = 64
+    powers = [-126, -100, -60, -20, -1, 0, 1, 20, 60, 100, 115, 127] if x_type == torch.bfloat16 else list(range(-14, 16, 3))
+    if w_fmt == 0:
+        powers = [p for p in powers if p <= 115]           # (16 + q) x has to stay a number
+    m = 40 if many else len(powers)
+    place = torch.tensor([r * 7 % k for r in range(m)], device="cuda")
+    exps = torch.tensor([powers[r % len(powers)] for r in range(m)], device="cuda")
+    x = torch.zeros((m, k), dtype=torch.float64, device="cuda")
+    x[torch.arange(m), place] = pow2(exps)
+    # column: one byte and one weight, the weight in every place of the row
+    byte, code = (t.flatten() for t in torch.meshgrid(torch.arange(256, device="cuda"), torch.arange(16, device="cuda"), indexing="ij"))
+    w = (code * 17).to(torch.uint8)[:, None].expand(-1, k // 2).contiguous()
+    s = byte.to(torch.uint8)[:, None].expand(-1, 2).contiguous()
+    y = pkg.gemv_w4(x.to(x_type), w, s, 32, w_fmt=w_fmt).double()
+    value = torch.tensor(E2M1 + [-t for t in E2M1], dtype=torch.float64, device="cuda")[code] if w_fmt == 1 else code.double() - 8.0
+    assert torch.isnan(y[:, byte == 255]).all()
+    want = pow2(exps)[:, None] * (value * pow2(byte - 127))[None, :]
+    ok = (byte < 255)[None, :] & ((want == 0) | ((want.abs() >= 2.0 ** -126) & (want.abs() < 2.0 ** 128)))
+    if w_fmt == 1 and x_type == torch.bfloat16:
+        ok &= ((value * pow2(byte - 127)).abs() < 2.0 ** 128)[None, :]        # as a bf16 number it would be an infinity
+    assert torch.equal(y[ok], want[ok]), "%d of %d differ" % (int((y[ok] != want[ok]).sum()), int(ok.sum()))
