@@ -273,7 +273,7 @@ int fp8gemm_launch_noalloc(int m, int k, int n, const void *a, int a_fmt, const 
 
 /*
  * ---- Internal: testing and tuning hooks --------------------------------------------
- * fp8gemm_launch_algo, fp8gemm_launch_tuned, fp8gemm_num_variants, fp8gemm_plan and
+ * fp8gemm_launch_algo, fp8gemm_launch_tuned, fp8gemm_num_variants, fp8gemm_plan, fp8gemm_w4_plan and
  * fp8gemm_tile_order expose the kernel families, their compiled variants and the planner
  * to the test suite and the tuning sweeps.  They are not part of the drop-in surface:
  * variant numbers, plan encodings and the set of variants change between versions.
@@ -306,6 +306,12 @@ int fp8gemm_grouped_tuned(int groups, int m, int k, int n, const int *row_offset
 int fp8gemm_grouped_wgrad_tuned(int groups, int rows, int m, int n, const int *row_offsets, const void *a_t, int a_fmt, const void *b_t,
                                 int b_fmt, int ld, void *out, int out_type, const float *a_scale, const float *b_scale,
                                 int accumulate, int variant, void *stream);
+
+/* How fp8gemm_gemv_w4 (groups 1) or fp8gemm_grouped_w4 lay a call out (pure host logic): plan[0] = rows of x at a time (16: the
+ * streaming kernel; 32 or 64: the one for more rows), plan[1] = waves along K, plan[2] = columns of a block, plan[3] = blocks
+ * that a workgroup goes through, plan[4] = how many of them have their scales staged at once (0: K in pieces; with more
+ * rows: the k whose scales are staged at once), plan[5] = rows an expert is taken to have at a time, plan[6] = slots of a wave's ring. */
+int fp8gemm_w4_plan(int groups, int m, int k, int n, int x_type, int w_fmt, int run, int scale_type, int plan[7]);
 
 /* Which family FP8GEMM_ALGO_AUTO picks for a shape (pure host logic). */
 int fp8gemm_select_algo(int m, int k, int n);

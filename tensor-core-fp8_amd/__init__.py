@@ -92,6 +92,8 @@ def lib():
     L.fp8gemm_select_algo.argtypes = [ci, ci, ci]
     L.fp8gemm_plan.restype = ci
     L.fp8gemm_plan.argtypes = [ci, ci, ci, ci, ctypes.POINTER(ci)]
+    L.fp8gemm_w4_plan.restype = ci
+    L.fp8gemm_w4_plan.argtypes = [ci, ci, ci, ci, ci, ci, ci, ci, ctypes.POINTER(ci)]
     L.fp8gemm_scratch_bytes.restype = ctypes.c_size_t
     L.fp8gemm_scratch_bytes.argtypes = [ci, ci, ci]
     L.fp8gemm_device_info.restype = ci
@@ -654,6 +656,15 @@ def gemm_grouped_wgrad(a_t, b_t, row_offsets, rows, a_scale=None, b_scale=None, 
             b_t.data_ptr(), _fp8_code(b_t, b_fmt), ld, out.data_ptr(), _wide_code(out.dtype), _floats(a_scale, groups * m, "a_scale"),
             _floats(b_scale, groups * n, "b_scale"), int(bool(accumulate)), variant)
     return out
+
+
+def w4_plan(m, k, n, x_type=T_BF16, w_fmt=W4_INT, run=128, scale_type=T_F16, groups=1):
+    """(rows at a time, waves along K, columns of a block, blocks of a workgroup, blocks or k staged at once, rows planned
+    for, ring slots) of a gemv_w4 call, as fp8gemm_w4_plan gives them."""
+    _sizes(m, k, n, groups)
+    out = (ctypes.c_int * 7)()
+    check(lib().fp8gemm_w4_plan(groups, m, k, n, x_type, w_fmt, run, scale_type, out))
+    return tuple(out)
 
 
 def gemv_w4(x, w, scales, run, w_fmt=W4_INT, zeros=None, x_scale=None, row_offsets=None, out_dtype=None, out=None, x_fmt=None,

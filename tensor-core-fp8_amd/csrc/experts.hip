@@ -103,11 +103,11 @@ int plan_wgrad(int rows, int m, int n, int groups)
 }  // namespace fp8gemm_detail
 
 namespace fp8gemm_detail {
-extern template hipError_t launch_w4<true, kW4Int>(const W4Args &, hipStream_t);
-extern template hipError_t launch_w4<false, kW4Int>(const W4Args &, hipStream_t);
-extern template hipError_t launch_w4<true, kW4Fp4>(const W4Args &, hipStream_t);
-extern template hipError_t launch_w4<false, kW4Fp4>(const W4Args &, hipStream_t);
-extern template hipError_t launch_w4<false, kW4Fp4Scaled>(const W4Args &, hipStream_t);
+extern template hipError_t launch_w4<true, kW4Int>(const W4Args &, hipStream_t, int *);
+extern template hipError_t launch_w4<false, kW4Int>(const W4Args &, hipStream_t, int *);
+extern template hipError_t launch_w4<true, kW4Fp4>(const W4Args &, hipStream_t, int *);
+extern template hipError_t launch_w4<false, kW4Fp4>(const W4Args &, hipStream_t, int *);
+extern template hipError_t launch_w4<false, kW4Fp4Scaled>(const W4Args &, hipStream_t, int *);
 }  // namespace fp8gemm_detail
 
 using namespace fp8gemm_detail;
@@ -229,7 +229,7 @@ bool quantize_source_ok(int rows, int cols, const void *x, int x_type, long long
 
 // ------------------------------------------------------------------ 4-bit weights
 int gemv_w4(int groups, int m, int k, int n, const int *row_offsets, const void *x, int x_type, const float *x_scale, const void *w, int w_fmt, int run,
-            const void *w_scales, int scale_type, const void *w_zeros, void *y, int y_type, void *stream)
+            const void *w_scales, int scale_type, const void *w_zeros, void *y, int y_type, void *stream, int *plan = nullptr)
 {
     if (groups <= 0 || groups > kMaxGroups || !size_ok(m) || !size_ok(k) || !size_ok(n) || run <= 0 || !x || !w || !w_scales || !y) return (int)hipErrorInvalidValue;
     if (run % 32 != 0 || k % run != 0 || k > (1 << 23)) return (int)hipErrorInvalidValue;
@@ -246,11 +246,11 @@ int gemv_w4(int groups, int m, int k, int n, const int *row_offsets, const void 
     const bool f16 = x_type != FP8GEMM_T_BF16;
     hipError_t e;
     if (w_fmt == FP8GEMM_W4_INT)
-        e = f16 ? launch_w4<true, kW4Int>(p, s) : launch_w4<false, kW4Int>(p, s);
+        e = f16 ? launch_w4<true, kW4Int>(p, s, plan) : launch_w4<false, kW4Int>(p, s, plan);
     else if (f16)
-        e = launch_w4<true, kW4Fp4>(p, s);
+        e = launch_w4<true, kW4Fp4>(p, s, plan);
     else
-        e = scale_type == FP8GEMM_T_E8M0 ? launch_w4<false, kW4Fp4Scaled>(p, s) : launch_w4<false, kW4Fp4>(p, s);
+        e = scale_type == FP8GEMM_T_E8M0 ? launch_w4<false, kW4Fp4Scaled>(p, s, plan) : launch_w4<false, kW4Fp4>(p, s, plan);
     return (int)e;
 }
 
@@ -338,6 +338,13 @@ int fp8gemm_grouped_w4(int groups, int m, int k, int n, const int *row_offsets, 
 {
     if (!row_offsets) return (int)hipErrorInvalidValue;
     return gemv_w4(groups, m, k, n, row_offsets, x, x_type, x_scale, w, w_fmt, run, w_scales, scale_type, w_zeros, y, y_type, stream);
+}
+
+int fp8gemm_w4_plan(int groups, int m, int k, int n, int x_type, int w_fmt, int run, int scale_type, int plan[7])
+{
+    if (!plan) return (int)hipErrorInvalidValue;
+    alignas(16) char some[16];                             // (stands for every operand: nothing is read)
+    return gemv_w4(groups, m, k, n, nullptr, some, x_type, nullptr, some, w_fmt, run, some, scale_type, nullptr, some, FP8GEMM_OUT_F32, nullptr, plan);
 }
 
 }  // extern "C"

@@ -36,9 +36,10 @@ struct W4Args {
 
 namespace fp8gemm_detail {
 
-// validated arguments -> kernel and launch (w4_pair.hip); the layout fields of `p` are filled in there
+// validated arguments -> kernel and launch (w4_pair.hip); the layout fields of `p` are filled in there.  With `plan` the
+// layout is written there (fp8gemm_w4_plan) and nothing is launched.
 template <bool F16, int MODE>
-hipError_t launch_w4(const W4Args &p, hipStream_t s);
+hipError_t launch_w4(const W4Args &p, hipStream_t s, int *plan);
 
 }  // namespace fp8gemm_detail
 

@@ -19,7 +19,7 @@ struct W4KernelTag {};
 constexpr int kW4MaxLds = 160 * 1024;
 
 template <bool F16, int MODE, int RUN, int KIND>
-hipError_t launch_w4_kernel(W4Args p, hipStream_t s)
+hipError_t launch_w4_kernel(W4Args p, hipStream_t s, int *plan)
 {
     // Rows of x that an expert has at a time, as far as the host can tell.
     const int busy = std::min(p.rows, p.groups);
@@ -70,6 +70,11 @@ hipError_t launch_w4_kernel(W4Args p, hipStream_t s)
         }
     if (best_lds == 0) return hipErrorInvalidValue;
     const int lds = best_lds, wc = kW4Waves >> p.wk_shift;
+    if (plan) {
+        const int layout[7] = {16, 1 << p.wk_shift, 16 * wc, p.blocks, p.pass, p.plan_rows, p.ring};
+        std::copy(layout, layout + 7, plan);
+        return hipSuccess;
+    }
     auto kernel = gemv_w4_kernel<F16, MODE, RUN, KIND>;
     hipError_t e = allow_lds<W4KernelTag<F16, MODE, RUN, KIND>>(kernel, kW4MaxLds);
     if (e != hipSuccess) return e;
@@ -81,7 +86,7 @@ template <bool F16, int MODE, int RUN, int MT, int KIND, int WK, int TN, bool CO
 struct W4WideKernelTag {};
 
 template <bool F16, int MODE, int RUN, int MT, int KIND, int WK, int TN, bool CODES>
-hipError_t launch_w4_wide(const W4Args &p, hipStream_t s)
+hipError_t launch_w4_wide(const W4Args &p, hipStream_t s, int *plan)
 {
     constexpr int COLS = w4_wide_cols(WK, TN), PIECE = w4_piece(WK), EB = w4_entry_bytes(MODE, KIND), ROOM = kW4MaxLds - w4_wide_x_bytes(MT, WK);
     // the scales of all of K, or of equal parts, whole turns of the weights' registers
@@ -93,6 +98,11 @@ hipError_t launch_w4_wide(const W4Args &p, hipStream_t s)
         scale_pieces = ((pieces + parts - 1) / parts + kW4Ahead - 1) / kW4Ahead * kW4Ahead;
         ++parts;
     } while (bytes(scale_pieces) > ROOM);
+    if (plan) {
+        const int layout[7] = {16 * MT, WK, COLS, 1, scale_pieces * PIECE, 0, 0};
+        std::copy(layout, layout + 7, plan);
+        return hipSuccess;
+    }
     auto kernel = gemm_w4_wide_kernel<F16, MODE, RUN, MT, KIND, WK, TN, CODES>;
     hipError_t e = allow_lds<W4WideKernelTag<F16, MODE, RUN, MT, KIND, WK, TN, CODES>>(kernel, kW4MaxLds);
     if (e != hipSuccess) return e;
@@ -101,7 +111,7 @@ hipError_t launch_w4_wide(const W4Args &p, hipStream_t s)
 }
 
 template <bool F16, int MODE, int RUN, int MT, int KIND>
-hipError_t launch_w4_tall(const W4Args &p, int busy, hipStream_t s)
+hipError_t launch_w4_tall(const W4Args &p, int busy, hipStream_t s, int *plan)
 {
     // Workgroups of 128 columns (two blocks of 16 a wave) where they still keep half the CUs busy (us for 64 / 128 columns: 64 x 4096 x
     // 16384 22.3 / 28.2, 32 x 4096 x 4096 15.2 / 21.8, 48 x 2048 x 24576 33.3 / 29.1, 17 x 8192 x 28672 49.0 / 40.7); else of 64; of 32
@@ -110,9 +120,9 @@ hipError_t launch_w4_tall(const W4Args &p, int busy, hipStream_t s)
     const long columns = (long)busy * p.n;
     auto launch = [&](auto codes) {
         constexpr bool CODES = decltype(codes)::value;
-        if (columns > 128 * 128) return launch_w4_wide<F16, MODE, RUN, MT, KIND, 2, 2, CODES>(p, s);
-        if (columns > 128 * 64 || p.k <= 1024) return launch_w4_wide<F16, MODE, RUN, MT, KIND, 2, 1, CODES>(p, s);
-        return launch_w4_wide<F16, MODE, RUN, MT, KIND, 4, 1, CODES>(p, s);
+        if (columns > 128 * 128) return launch_w4_wide<F16, MODE, RUN, MT, KIND, 2, 2, CODES>(p, s, plan);
+        if (columns > 128 * 64 || p.k <= 1024) return launch_w4_wide<F16, MODE, RUN, MT, KIND, 2, 1, CODES>(p, s, plan);
+        return launch_w4_wide<F16, MODE, RUN, MT, KIND, 4, 1, CODES>(p, s, plan);
     };
     if constexpr (F16)
         if (p.x_type != FP8GEMM_T_F16) return launch(std::true_type{});
@@ -120,28 +130,28 @@ hipError_t launch_w4_tall(const W4Args &p, int busy, hipStream_t s)
 }
 
 template <bool F16, int MODE, int RUN, int KIND>
-hipError_t launch_w4_rows(const W4Args &p, hipStream_t s)
+hipError_t launch_w4_rows(const W4Args &p, hipStream_t s, int *plan)
 {
     // Rows of x per pass over the weights; with experts, what an expert has on average (eight experts, us for gemv / 32 rows at a
     // time: 4096 x 4096 integers, 8 rows each 23.2 / 25.2, 12 rows 30.6 / 25.1; 2048 x 2048 e2m1, 8 rows 16.2 / 9.9).
     const int busy = std::min(p.rows, p.groups), average = (p.rows + busy - 1) / busy;
-    if (p.rows <= 16 || average <= 6) return launch_w4_kernel<F16, MODE, RUN, KIND>(p, s);
-    return p.rows <= 32 || average <= 16 ? launch_w4_tall<F16, MODE, RUN, 2, KIND>(p, busy, s) : launch_w4_tall<F16, MODE, RUN, 4, KIND>(p, busy, s);
+    if (p.rows <= 16 || average <= 6) return launch_w4_kernel<F16, MODE, RUN, KIND>(p, s, plan);
+    return p.rows <= 32 || average <= 16 ? launch_w4_tall<F16, MODE, RUN, 2, KIND>(p, busy, s, plan) : launch_w4_tall<F16, MODE, RUN, 4, KIND>(p, busy, s, plan);
 }
 
 template <bool F16, int MODE>
-hipError_t launch_w4(const W4Args &p, hipStream_t s)
+hipError_t launch_w4(const W4Args &p, hipStream_t s, int *plan)
 {
     const bool long_runs = p.run % 128 == 0;
     if constexpr (MODE == kW4Fp4Scaled) {
-        return long_runs ? launch_w4_rows<F16, MODE, 128, kW4ScaleByte>(p, s) : launch_w4_rows<F16, MODE, 32, kW4ScaleByte>(p, s);
+        return long_runs ? launch_w4_rows<F16, MODE, 128, kW4ScaleByte>(p, s, plan) : launch_w4_rows<F16, MODE, 32, kW4ScaleByte>(p, s, plan);
     } else {
-        if (p.scale_type == FP8GEMM_T_F32) return long_runs ? launch_w4_rows<F16, MODE, 128, kW4ScaleF32>(p, s) : launch_w4_rows<F16, MODE, 32, kW4ScaleF32>(p, s);
-        if (p.scale_type == FP8GEMM_T_F16) return long_runs ? launch_w4_rows<F16, MODE, 128, kW4ScaleF16>(p, s) : launch_w4_rows<F16, MODE, 32, kW4ScaleF16>(p, s);
-        return long_runs ? launch_w4_rows<F16, MODE, 128, kW4ScaleBf16>(p, s) : launch_w4_rows<F16, MODE, 32, kW4ScaleBf16>(p, s);
+        if (p.scale_type == FP8GEMM_T_F32) return long_runs ? launch_w4_rows<F16, MODE, 128, kW4ScaleF32>(p, s, plan) : launch_w4_rows<F16, MODE, 32, kW4ScaleF32>(p, s, plan);
+        if (p.scale_type == FP8GEMM_T_F16) return long_runs ? launch_w4_rows<F16, MODE, 128, kW4ScaleF16>(p, s, plan) : launch_w4_rows<F16, MODE, 32, kW4ScaleF16>(p, s, plan);
+        return long_runs ? launch_w4_rows<F16, MODE, 128, kW4ScaleBf16>(p, s, plan) : launch_w4_rows<F16, MODE, 32, kW4ScaleBf16>(p, s, plan);
     }
 }
 
-template hipError_t launch_w4<FP8GEMM_W4_F16 != 0, FP8GEMM_W4_MODE>(const W4Args &, hipStream_t);
+template hipError_t launch_w4<FP8GEMM_W4_F16 != 0, FP8GEMM_W4_MODE>(const W4Args &, hipStream_t, int *);
 
 }  // namespace fp8gemm_detail

@@ -95,3 +95,42 @@ def w4_values(w, scales, run, w_fmt, zeros=None):
         v = q.double() - z
     s = scale_values(scales)
     return v * s.repeat_interleave(run, -1)
+
+
+# Products with 4-bit weights that between them take every kind of layout of the streaming kernel: 1, 2, 4 and 8 waves along K, one
+# block of columns a workgroup and several, whose scales are staged one, several or all at a time, K in pieces, two and four
+# ring slots.  (groups, m, k, n, x type, weights, run, scale type, layout as w4_plan gives it)
+W4_LAYOUTS = [
+    (1, 12, 512, 120000, 1, 0, 32, 0, (16, 1, 128, 2, 1, 12, 2)),
+    (3, 4, 128, 28672, 1, 0, 128, 2, (16, 1, 128, 2, 2, 2, 2)),
+    (1, 1, 128, 120000, 1, 0, 128, 2, (16, 1, 128, 2, 2, 1, 4)),
+    (3, 4, 128, 120000, 1, 0, 32, 0, (16, 1, 128, 6, 4, 2, 2)),
+    (1, 7, 1024, 120000, 1, 0, 32, 0, (16, 1, 128, 2, 0, 7, 2)),
+    (1, 12, 128, 16, 1, 0, 32, 0, (16, 1, 128, 1, 1, 12, 2)),
+    (1, 1, 128, 16, 1, 0, 128, 2, (16, 1, 128, 1, 1, 1, 4)),
+    (1, 16, 2048, 28672, 1, 0, 32, 0, (16, 1, 128, 1, 0, 16, 2)),
+    (3, 4, 2048, 28672, 1, 0, 32, 0, (16, 2, 64, 3, 1, 2, 2)),
+    (3, 4, 2048, 28672, 1, 0, 128, 2, (16, 2, 64, 3, 3, 2, 2)),
+    (3, 4, 2048, 28672, 1, 0, 32, 2, (16, 2, 64, 3, 2, 2, 2)),
+    (3, 4, 4096, 28672, 1, 0, 32, 2, (16, 2, 64, 3, 0, 2, 2)),
+    (8, 16, 1024, 1100, 1, 0, 32, 2, (16, 2, 64, 1, 1, 2, 2)),
+    (1, 1, 2048, 17000, 1, 0, 128, 2, (16, 2, 64, 1, 1, 1, 4)),
+    (3, 12, 4096, 8192, 1, 0, 32, 0, (16, 2, 64, 1, 0, 4, 2)),
+    (1, 12, 4096, 17000, 1, 0, 32, 2, (16, 4, 32, 3, 1, 12, 2)),
+    (1, 16, 2048, 17000, 1, 0, 32, 0, (16, 4, 32, 3, 3, 16, 2)),
+    (1, 4, 4096, 17000, 1, 0, 32, 2, (16, 4, 32, 3, 3, 4, 4)),
+    (1, 7, 4096, 17000, 1, 0, 32, 0, (16, 4, 32, 3, 2, 7, 2)),
+    (32, 24, 14336, 2048, 1, 0, 128, 2, (16, 4, 32, 3, 0, 1, 2)),
+    (1, 4, 1024, 16, 1, 0, 32, 2, (16, 4, 32, 1, 1, 4, 2)),
+    (1, 1, 1024, 16, 1, 0, 128, 2, (16, 4, 32, 1, 1, 1, 4)),
+    (1, 12, 4096, 8192, 1, 0, 32, 0, (16, 4, 32, 1, 0, 12, 2)),
+    (8, 40, 8192, 1100, 1, 0, 32, 0, (16, 8, 16, 3, 1, 5, 2)),
+    (1, 1, 14336, 17000, 1, 0, 32, 0, (16, 8, 16, 5, 1, 1, 4)),
+    (1, 2, 4096, 17000, 1, 0, 32, 2, (16, 8, 16, 3, 3, 2, 2)),
+    (1, 4, 8192, 17000, 1, 0, 128, 2, (16, 8, 16, 5, 5, 4, 4)),
+    (1, 1, 4096, 17000, 1, 0, 32, 0, (16, 8, 16, 3, 2, 1, 2)),
+    (8, 16, 28672, 1100, 1, 0, 32, 2, (16, 8, 16, 3, 0, 2, 2)),
+    (1, 2, 2048, 16, 1, 0, 32, 0, (16, 8, 16, 1, 1, 2, 2)),
+    (1, 1, 2048, 16, 1, 0, 128, 2, (16, 8, 16, 1, 1, 1, 4)),
+    (1, 16, 4096, 16, 1, 0, 128, 2, (16, 8, 16, 1, 0, 16, 2)),
+]

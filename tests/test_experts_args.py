@@ -125,3 +125,22 @@ def test_sizes_that_an_int_cuts_off(pkg):
     a = torch.empty((4, 64), dtype=torch.float8_e4m3fn, device="meta")
     with pytest.raises(pkg.Fp8GemmError):
         pkg.GEMM(4, 64, WRAPS, a, a, a)
+
+
+def test_w4_layouts(pkg):
+    """The calls that the GPU tests make to reach every layout still reach it (a host decision)."""
+    from expert_util import W4_LAYOUTS
+    kinds = set()
+    for groups, m, k, n, x_type, w_fmt, run, scale, layout in W4_LAYOUTS:
+        assert pkg.w4_plan(m, k, n, x_type, w_fmt, run, scale, groups) == layout
+        rows, wk, cols, blocks, at_once, planned, ring = layout
+        assert rows == 16 and wk * cols == 128 and ring in (2, 4) and planned <= 16
+        kinds.add((wk, "pieces" if at_once == 0 else ("one" if blocks == 1 else ("all" if at_once >= blocks else ("several" if at_once > 1 else "each")))))
+    assert kinds >= {(wk, kind) for wk in (1, 2, 4, 8) for kind in ("pieces", "one", "all", "each")}
+    assert {(wk, "several") for wk in (1, 2, 4, 8)} <= kinds
+    # more rows: 32 or 64 at a time, the scales of all of K or of a part
+    assert pkg.w4_plan(17, 4096, 4096)[0] == 32 and pkg.w4_plan(33, 4096, 4096)[0] == 64 and pkg.w4_plan(64, 4096, 4096, groups=8)[0] == 32
+    assert pkg.w4_plan(64, 28672, 129, run=32, scale_type=pkg.T_F32)[4] < 28672 <= pkg.w4_plan(64, 28672, 129, run=128)[4]
+    for bad in (dict(m=0, k=256, n=64), dict(m=1, k=256, n=64, run=48), dict(m=1, k=256, n=64, groups=2000), dict(m=1, k=256, n=64, x_type=0)):
+        with pytest.raises(pkg.Fp8GemmError):
+            pkg.w4_plan(**bad)
