@@ -495,12 +495,14 @@ def _launch(fn, index, stream, *args):
         check(code)
 
 
-def _floats(t, count, what):
-    """Pointer to `count` contiguous float32 device elements, or None."""
+def _floats(t, count, what, groups=0):
+    """Pointer to `count` contiguous float32 device elements, or None; a matrix of them has a row for each of `groups`."""
     if t is None:
         return None
     if t.dtype is not _torch.float32 or t.numel() != count or not t.is_contiguous():
         raise Fp8GemmError("%s: expected %d contiguous float32 elements" % (what, count))
+    if groups and t.dim() > 1 and t.shape[0] != groups:
+        raise Fp8GemmError("%s: expected a row for each of %d experts, got %s" % (what, groups, tuple(t.shape)))
     return t.data_ptr()
 
 
@@ -624,7 +626,7 @@ def gemm_grouped(a, b, row_offsets, a_scale=None, b_scale=None, out_dtype=None, 
     per_column = b_scale is not None and b_scale.dim() == 2
     _launch(L.fp8gemm_grouped_tuned, device, stream, groups, m, k, n, offs, a.data_ptr(), _fp8_code(a, a_fmt), b.data_ptr(),
             _fp8_code(b, b_fmt), out.data_ptr(), _wide_code(out.dtype), _floats(a_scale, m, "a_scale"),
-            _floats(b_scale, groups * n if per_column else groups, "b_scale"), int(per_column), variant)
+            _floats(b_scale, groups * n if per_column else groups, "b_scale", groups if per_column else 0), int(per_column), variant)
     return out
 
 
@@ -653,8 +655,8 @@ def gemm_grouped_wgrad(a_t, b_t, row_offsets, rows, a_scale=None, b_scale=None, 
             _fill(out, 0.0, stream)
         return out
     _launch(L.fp8gemm_grouped_wgrad_tuned, device, stream, groups, rows, m, n, offs, a_t.data_ptr(), _fp8_code(a_t, a_fmt),
-            b_t.data_ptr(), _fp8_code(b_t, b_fmt), ld, out.data_ptr(), _wide_code(out.dtype), _floats(a_scale, groups * m, "a_scale"),
-            _floats(b_scale, groups * n, "b_scale"), int(bool(accumulate)), variant)
+            b_t.data_ptr(), _fp8_code(b_t, b_fmt), ld, out.data_ptr(), _wide_code(out.dtype), _floats(a_scale, groups * m, "a_scale", groups),
+            _floats(b_scale, groups * n, "b_scale", groups), int(bool(accumulate)), variant)
     return out
 
 

@@ -144,3 +144,16 @@ def test_w4_layouts(pkg):
     for bad in (dict(m=0, k=256, n=64), dict(m=1, k=256, n=64, run=48), dict(m=1, k=256, n=64, groups=2000), dict(m=1, k=256, n=64, x_type=0)):
         with pytest.raises(pkg.Fp8GemmError):
             pkg.w4_plan(**bad)
+
+
+def test_scales_lie_by_expert(pkg):
+    """A matrix of scales with its axes exchanged holds as many numbers: refused, not read as if it were the other one."""
+    import torch
+    pkg._setup()
+    good = torch.ones((4, 6))
+    assert pkg._floats(good, 24, "b_scale", 4) == good.data_ptr()
+    assert pkg._floats(good.view(24), 24, "b_scale", 4) == good.data_ptr()
+    assert pkg._floats(torch.ones((24, 1)), 24, "a_scale") and pkg._floats(None, 24, "a_scale", 4) is None
+    for bad in (torch.ones((6, 4)), torch.ones((1, 24)), torch.ones((4, 5)), good.t(), good.double()):
+        with pytest.raises(pkg.Fp8GemmError):
+            pkg._floats(bad, 24, "b_scale", 4)

@@ -411,3 +411,15 @@ def test_wgrad_scales_of_experts_without_tokens(pkg, n, dtype):
                     assert not out[g].view(bits).any(), (variant, g)
                     assert torch.equal(into[g].view(bits), held[g].view(bits)), (variant, g)
             check_wgrad(out[[1, 4]], [at[1], at[4]], [cs[1], cs[4]], a, b, None if x is None else x[[1, 4]], None if y is None else y[[1, 4]], dtype)
+
+
+def test_scales_with_exchanged_axes_are_refused(pkg):
+    gen = generator("axes")
+    off, a, b = case(gen, [3, 0, 5], 128, 64, 0, 0)
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg.gemm_grouped(a, b, off, b_scale=powers(gen, 64, 3))
+    _, at, _, _ = transposed(gen, [3, 0, 5], 48, 0)
+    _, bt, _, _ = transposed(gen, [3, 0, 5], 64, 0)
+    for sa, sb in ((powers(gen, 48, 3), None), (None, powers(gen, 64, 3))):
+        with pytest.raises(pkg.Fp8GemmError):
+            pkg.gemm_grouped_wgrad(at, bt, off, 8, a_scale=sa, b_scale=sb)
