@@ -577,8 +577,13 @@ def quantize_rows(x, fmt=E4M3, row_index=None, codes=None, scales=None, stream=N
     scales = _output(scales, (rows,), _torch.float32, x, stream)
     if rows == 0:
         return codes, scales
-    _launch(L.fp8gemm_quantize_rows, device, stream, rows, cols, x.data_ptr(), x_type, stride, x_rows,
-            None if row_index is None else _ints(row_index, "row_index"), fmt, codes.data_ptr(), scales.data_ptr())
+    index = None if row_index is None else _ints(row_index, "row_index")
+    if x_rows == 0 and cols > 0:              # every index is outside x
+        _fill(codes.view(_torch.uint8), 0, stream)
+        _fill(scales, 1.0, stream)
+        return codes, scales
+    _launch(L.fp8gemm_quantize_rows, device, stream, rows, cols, x.data_ptr(), x_type, stride, x_rows, index, fmt, codes.data_ptr(),
+            scales.data_ptr())
     return codes, scales
 
 
@@ -596,8 +601,13 @@ def quantize_columns(x, row_offsets, fmt=E4M3, row_index=None, codes=None, scale
     if rows == 0:
         _fill(scales, 1.0, stream)
         return codes, scales
-    _launch(L.fp8gemm_quantize_columns, device, stream, groups, rows, cols, offs, x.data_ptr(), x_type, stride, x_rows,
-            None if row_index is None else _ints(row_index, "row_index"), fmt, codes.data_ptr(), ld, scales.data_ptr())
+    index = None if row_index is None else _ints(row_index, "row_index")
+    if x_rows == 0 and cols > 0 and ld > 0:   # every index is outside x
+        _fill(codes.view(_torch.uint8), 0, stream)
+        _fill(scales, 1.0, stream)
+        return codes, scales
+    _launch(L.fp8gemm_quantize_columns, device, stream, groups, rows, cols, offs, x.data_ptr(), x_type, stride, x_rows, index, fmt,
+            codes.data_ptr(), ld, scales.data_ptr())
     return codes, scales
 
 

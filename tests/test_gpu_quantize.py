@@ -285,3 +285,29 @@ def test_split_columns_captured_and_replayed(pkg):
         want, want_s = pkg.quantize_columns(x, off)
         assert torch.equal(codes.view(torch.uint8), want.view(torch.uint8)) and torch.equal(scales, want_s)
         check_columns(pkg, x, counts, 0)
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+def test_indices_into_nothing(pkg, fmt):
+    """A padded batch that has no token: every index is outside a matrix without rows, and stands for a row of zeros."""
+    x = torch.empty((0, 200), dtype=torch.bfloat16, device="cuda")
+    index = torch.full((70,), -1, dtype=torch.int32, device="cuda")
+    off = offsets_of([40, 0, 30])
+    for stream in (None, torch.cuda.Stream()):
+        c, s = torch.full((70, 200), 3.0, device="cuda").to(F8[fmt]), torch.full((70,), 5.0, device="cuda")
+        torch.cuda.synchronize()
+        assert pkg.quantize_rows(x, fmt, row_index=index, codes=c, scales=s, stream=stream) == (c, s)
+        ct, st = pkg.quantize_columns(x, off, fmt, row_index=index, stream=stream)
+        torch.cuda.synchronize()
+        assert not c.view(torch.uint8).any() and (s == 1).all()
+        assert ct.shape == (200, pkg.grouped_ld(70, 3)) and not ct.view(torch.uint8).any() and st.shape == (3, 200) and (st == 1).all()
+    # the same from a matrix that has rows
+    some = torch.ones((5, 200), dtype=torch.bfloat16, device="cuda")
+    want = pkg.quantize_columns(some, off, fmt, row_index=index)
+    assert torch.equal(want[0].view(torch.uint8), ct.view(torch.uint8)) and torch.equal(want[1], st)
+    # an index is checked all the same
+    for bad in (index.long(), index.cpu(), index[::2]):
+        with pytest.raises(pkg.Fp8GemmError):
+            pkg.quantize_rows(x, fmt, row_index=bad)
+        with pytest.raises(pkg.Fp8GemmError):
+            pkg.quantize_columns(x, off, fmt, row_index=bad)
