@@ -533,6 +533,8 @@ def _output(out, shape, dtype, like, stream):
 
 
 def _fill(t, value, stream):
+    if stream is not None and stream.device.index != t.get_device():
+        raise Fp8GemmError("the stream belongs to another device than the operands")
     with _torch.cuda.stream(stream):
         t.fill_(value)
 

@@ -157,3 +157,19 @@ def test_scales_lie_by_expert(pkg):
     for bad in (torch.ones((6, 4)), torch.ones((1, 24)), torch.ones((4, 5)), good.t(), good.double()):
         with pytest.raises(pkg.Fp8GemmError):
             pkg._floats(bad, 24, "b_scale", 4)
+
+
+def test_results_without_a_kernel_go_by_their_stream_too(pkg):
+    """A stream of another device is refused where an empty batch needs no launch, as it is where there is one."""
+    import torch
+
+    class Stream:
+        device = torch.device("cuda", 5)
+
+    pkg._setup()
+    t = torch.ones(3)
+    with pytest.raises(pkg.Fp8GemmError):
+        pkg._fill(t, 0.0, Stream())
+    assert (t == 1).all()
+    pkg._fill(t, 2.0, None)
+    assert (t == 2).all()
