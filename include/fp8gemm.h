@@ -144,7 +144,8 @@ void fp8gemm_sorted_row_swizzle(int m, const int *row_offsets, int *row_indices)
  * the same array.  Offsets outside the matrix are clamped to it and one below an earlier one is raised
  * to it; no content of the array makes a call leave its operands.  Rows in front of the first expert and
  * behind the last one are left as they are.  None of the calls allocates or uses scratch.  Sizes are 1 .. 2^30 (a
- * transposed operand's row: up to 2^23); outputs must not overlap inputs.  There is no counterpart in the reference.
+ * transposed operand's row: up to 2^23), and a call that takes more workgroups than a grid of 2^32 threads holds is refused
+ * (one workgroup of 64 threads for 32 x 32 outputs where the tiled kernels do not run); outputs must not overlap inputs.  There is no counterpart in the reference.
  *
  * fp8gemm_grouped: for every row i of expert g and every j < n
  *     out[i * n + j] = cast( a_scale[i] * b_scale * sum_{t<k} a[i * k + t] * b[(g * n + j) * k + t] )

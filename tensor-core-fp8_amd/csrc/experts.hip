@@ -170,8 +170,9 @@ hipError_t launch_quantize_rows(int rows, int cols, const void *x, size_t stride
     hipLaunchKernelGGL((quantize_rows_kernel<TYPE, FMT, WAVES, HELD>), dim3((unsigned)((now + 4 / WAVES - 1) / (4 / WAVES))), dim3(256), 0, s, \
                        now, cols, x, stride, x_rows, index, codes, scales)
         // Four waves to a row, two or eight pieces of eight elements a lane; short rows get a wave each, for which four would be
-        // half idle.  One wave with eight pieces for rows of 4096 is slower: 32768 rows 109 us against 97, 3001 rows of
-        // 2048 11.6 against 9.8 (other data read in between, so that x is not cached).
+        // half idle.  One wave with eight pieces for rows of up to 4096 is slower: 32768 rows of 4096 74.4 us against 68.0 (calls
+        // one behind the other on three matrices), 3001 rows of 2048 8.0 against 7.7; but rows that are not whole pieces 16.2
+        // against 18.0 (8192 of 1843).
         if (cols <= 1024)
             ROWS_KERNEL(1, 2);
         else if (cols <= 4096)

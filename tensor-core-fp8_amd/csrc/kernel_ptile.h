@@ -862,7 +862,8 @@ __device__ __forceinline__ void gemm_ptile_body(int M, int K, int N,
                     v4f buf[NR], fb = {1.0f, 1.0f, 1.0f, 1.0f};
                     float fa[NR];
                     if (!quads || grp.accumulate) {
-                        // single elements, or C read back: a few rows at a time
+                        // single elements, or C read back: a few rows at a time (slow: 16 matrices of 8192 x 4096 bf16 added to 3.2 ms,
+                        // written 0.98; 8192 rows times 4095 columns 158 us, 4096 122)
 #pragma unroll 1
                         for (int r0 = 0; r0 < 32; r0 += RPI_ST) {
                             const v4f v = *reinterpret_cast<const v4f *>(stg + (r0 + rl) * ROWB + cl * 16);

@@ -121,7 +121,7 @@ __device__ __forceinline__ bool quant_fold(float x, uint32_t &amax_bits)
 // Row r of codes = row (row_index ? row_index[r] : r) of x; a row_index outside [0, x_rows) gives a row of zeros with
 // scale 1.  WAVES waves to a row, 4 / WAVES rows to a workgroup.  HBM bound: every wide element is read once, held in
 // registers (HELD pieces of eight elements a lane) until the row's maximum is known, and its code written: 32768 rows
-// of 4096 bf16 take 70 us, gathered from 16384 74, 8192 rows of 1843 16.5.
+// of 4096 bf16 that no cache holds take 62 us (6.5 TB/s), gathered from 16384 67, 8192 rows of 1843 18.
 template <int TYPE, int FMT, int WAVES, int HELD>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(int rows, int cols, const void *__restrict__ x, size_t x_stride, int x_rows,
                                                             const int *__restrict__ row_index, uint8_t *__restrict__ codes, float *__restrict__ scales)
@@ -192,7 +192,8 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(int rows, int cols, 
     if (lane == 0 && sub == 0) scales[row] = quant_scale(e);
 }
 
-// The same for any row length: a workgroup to a row, which is read twice.
+// The same for any row length: a workgroup to a row, which is read twice, an element a lane and load: 4096 rows of 28672 bf16
+// 223 us, a single one 35, where 4096 rows of 16384 take 34 above.
 template <int TYPE, int FMT>
 __global__ __launch_bounds__(256) void quantize_rows_any_kernel(int cols, const void *__restrict__ x, size_t x_stride, int x_rows,
                                                                 const int *__restrict__ row_index, uint8_t *__restrict__ codes, float *__restrict__ scales)
@@ -239,8 +240,8 @@ __global__ __launch_bounds__(256) void quantize_rows_any_kernel(int cols, const 
 // columns (a line of 16-bit numbers) of one group, 256 or 512 rows at a time, quads of rows of eight columns a thread: a first walk
 // finds the maxima, the second one goes backwards, so that it starts with the rows that are still in registers (all of
 // them, for a group of no more rows) and goes on with those that are still cached.  128 x 64 pieces are turned
-// around in LDS, so that every column's 128 codes leave as one whole line.  32768 rows of 4096 bf16 in 32 groups: 120 us, 3.4 TB/s
-// (half of the rows are read a second time), 4099 rows of 2048 in 8: 16.
+// around in LDS, so that every column's 128 codes leave as one whole line.  32768 rows of 4096 bf16 in 32 uneven groups: 125 us, 5 TB/s
+// of the 625 MB that move (three quarters of the rows are read a second time; 108 us in even groups), 4099 rows of 2048 in 8: 15.
 constexpr int kColBlock = 64;
 constexpr int kColThreads = 512;
 // rows at a time: four or eight a thread, which are 32 registers of either

@@ -22,7 +22,8 @@
 // A workgroup of eight waves is WC waves side by side (16 columns each) times WK waves along K, whose sums are
 // added in wave order through LDS: few columns still fill the chip.  It goes through several blocks of columns;
 // x and the scales of all of them are staged in LDS once, then the waves' rings run without a break over all blocks.
-// One row, 28672 x 8192 integers in runs of 128: 27 us, 4.5 TB/s; runs of 32 38 us, where the vector unit is the bound.
+// One row, 28672 x 8192 integers in runs of 128: 27 us, 4.5 TB/s; runs of 32 37 us.  By the counters the vector unit is what is
+// busiest, 64 and 70 % of the CUs' time, start and end of the launch included (matrix unit 28 and 18, LDS 26 and 30).
 #ifndef FP8GEMM_KERNEL_W4_H
 #define FP8GEMM_KERNEL_W4_H
 
@@ -596,10 +597,11 @@ __global__ __launch_bounds__(64 * kW4Waves, 4) void gemv_w4_kernel(W4Args p)
 // where the columns are few.
 //
 // Where the four lanes of a row have to share 32 consecutive weights (see above) their 16-byte loads are turned around by
-// swaps between lanes.  64 rows, integers in runs of 128: 4096 x 4096 18 us (the kernel above, in blocks of 64 rows, 69),
+// swaps between lanes.  64 rows, integers in runs of 128: 4096 x 4096 17 us (the kernel above, in blocks of 64 rows, 69),
 // 17536 x 6784 with 58 rows 55 (100): the matrix unit, LDS and the vector unit take 0.4 to 0.8 us of a piece's 1.7 each, and two
 // waves on a SIMD in step overlap little of it.  Reading x a step ahead, or starting every workgroup at another piece, gains
-// nothing.
+// nothing.  What few columns cost besides is idle CUs: 64 rows of 4096 x 4096 have 128 workgroups, and the blocks of an expert's
+// rows go by one behind the other in the same ones (1024 rows of 4096 x 4096 238 us).
 constexpr int kW4Ahead = 4;
 // WK waves along K: a piece has 128 k of each, a workgroup 16 * TN columns of the others side by side
 __host__ __device__ constexpr int w4_piece(int wk) { return 128 * wk; }

@@ -30,7 +30,9 @@ hipError_t launch_w4_kernel(W4Args p, hipStream_t s, int *plan)
     // stage the rows of x or where not all of x fits, and two workgroups on a CU hide 28 % of each other's time.  The experts that
     // will have rows are counted as if every row fell on any of them.  Fitted to 140 calls (integers in runs of 32 and 128, e2m1, 1 to
     // 14 rows of one matrix, 8 to 40 of 8 and 32 experts): the pick takes 0.7 % longer than the best of the eight layouts on
-    // average, 12 % at worst.
+    // average, 12 % at worst.  Not among them, and slower than by the fit to fewer calls before it: 2 rows of 8192 x 28672 in runs of
+    // 128 35.0 us (31.0), 8 rows of 28672 x 8192 35.9 (34.8); faster: 1 row of 28672 x 8192 in runs of 32 36.8 (43.6), 4 rows in runs
+    // of 128 30.9 (33.9).
     constexpr int EB = w4_entry_bytes(MODE, KIND);
     const double active = p.groups > 1 ? p.groups * (1.0 - std::pow(1.0 - 1.0 / p.groups, p.rows)) : 1.0;
     double best = 1e30;
@@ -133,7 +135,8 @@ template <bool F16, int MODE, int RUN, int KIND>
 hipError_t launch_w4_rows(const W4Args &p, hipStream_t s, int *plan)
 {
     // Rows of x per pass over the weights; with experts, what an expert has on average (eight experts, us for gemv / 32 rows at a
-    // time: 4096 x 4096 integers, 8 rows each 23.2 / 25.2, 12 rows 30.6 / 25.1; 2048 x 2048 e2m1, 8 rows 16.2 / 9.9).
+    // time: 4096 x 4096 integers, 8 rows each 23.2 / 25.2, 12 rows 30.6 / 25.1; 2048 x 2048 e2m1, 8 rows 16.2 / 9.9).  The host knows no more than the average: 192 rows to 32
+    // experts of 4096 x 4096 take 54 us in even parts and 390 all to one, whose weights are read for every 16 of them.
     const int busy = std::min(p.rows, p.groups), average = (p.rows + busy - 1) / busy;
     if (p.rows <= 16 || average <= 6) return launch_w4_kernel<F16, MODE, RUN, KIND>(p, s, plan);
     return p.rows <= 32 || average <= 16 ? launch_w4_tall<F16, MODE, RUN, 2, KIND>(p, busy, s, plan) : launch_w4_tall<F16, MODE, RUN, 4, KIND>(p, busy, s, plan);
