@@ -218,3 +218,42 @@ def test_sizes_that_an_int_cuts_off(pkg):
     w = flat.view(torch.uint8)[:, :wraps // 2]
     with pytest.raises(pkg.Fp8GemmError):
         pkg.gemv_w4(flat, w, torch.empty((1, wraps // 256), device="cuda"), 256)
+
+
+@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("rows,experts,cols", [(300, 4, 96), (300, 70, 40), (5000, 2, 64)])
+def test_offsets_that_are_no_cut(pkg, rows, experts, cols, seed):
+    """Offsets below zero, beyond the rows and out of order, some experts in front of the first row of the others: every
+    operator goes by the same cut, each offset clamped to the rows and raised to the largest before it."""
+    gen = generator("no cut", rows, experts, seed)
+    bad = torch.randint(-rows // 3, rows + rows // 3, (experts + 1,), generator=gen, device="cuda")
+    if seed % 2:
+        bad = torch.sort(bad).values + torch.randint(-9, 10, (experts + 1,), generator=gen, device="cuda")
+    meant = torch.cummax(bad.clamp(0, rows), 0).values.to(torch.int32)
+    bad = bad.to(torch.int32)
+    x = torch.randn((rows, cols), generator=gen, device="cuda").to(torch.bfloat16)
+    dy = torch.randn((rows, 136), generator=gen, device="cuda").to(torch.float16)
+    got = [pkg.quantize_columns(t, bad, fmt) for t, fmt in ((x, pkg.E4M3), (dy, pkg.E5M2))]
+    want = [pkg.quantize_columns(t, meant, fmt) for t, fmt in ((x, pkg.E4M3), (dy, pkg.E5M2))]
+    for (c, s), (c2, s2) in zip(got, want):
+        assert torch.equal(c.view(torch.uint8), c2.view(torch.uint8)) and torch.equal(s, s2)
+    off = meant.tolist()
+    at, counts, used = places(off, rows)
+    (xc, xs), (yc, ys) = got
+    assert not xc.view(torch.uint8)[:, used:].any()
+    dw = pkg.gemm_grouped_wgrad(yc, xc, bad, rows, a_scale=ys, b_scale=xs)
+    for g, (p, c) in enumerate(zip(at, counts)):
+        y, tol = fp8_product(yc[:, p:p + c].double(), xc[:, p:p + c].double()) if c else (torch.zeros_like(dw[g], dtype=torch.float64),) * 2
+        f = ys[g][:, None].double() * xs[g].double()
+        assert ((dw[g].double() - y * f).abs() <= tol * f + rounding(y * f, torch.float32) * 1.0001).all()
+    # 4-bit matrices, with the kernel for few rows an expert and the one for many
+    n, k, run = 48, 64, 32
+    w = torch.randint(0, 256, (experts, n, k // 2), generator=gen, dtype=torch.uint8, device="cuda")
+    s = torch.ones((experts, n, k // run), device="cuda")
+    h = torch.randint(-3, 4, (rows, k), generator=gen, device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    y = torch.full((rows, n), 9.0, device="cuda")
+    pkg.gemv_w4(h, w, s, run, row_offsets=bad, out=y)
+    for g in range(experts):
+        lo, hi = off[g], off[g + 1]
+        assert hi == lo or torch.equal(y[lo:hi].double(), h[lo:hi].double() @ w4_values(w[g], s[g], run, 0).t().contiguous())
+    assert (y[:off[0]] == 9.0).all() and (y[off[-1]:] == 9.0).all()
